@@ -20,6 +20,8 @@ if os.environ.get("GVK_LIBRARY"):
 
 GVK_OK, GVK_EINVAL, GVK_EDIM, GVK_EHIP, GVK_ENOMEM = 0, -1, -2, -3, -4
 SGD, MOMENTUM, ADAGRAD, RMSPROP, ADAM = range(5)
+F32, BF16, F16 = range(3)
+MAX_BLOCK_DIM = 4096
 TUNE_LANES_PER_PAIR = 1
 TUNE_VARIANT = 2
 TUNE_RUN_CAP = 3
@@ -156,6 +158,25 @@ def lib():
                                           i32, i32, f32, vp, C.c_size_t, u32, u32, i32, i32, i32, i32, i32, i32]
     l.gvk_predict.restype = i32
     l.gvk_predict.argtypes = [vp, i32, vp, vp, vp, vp, i32]
+    wide = C.c_int64  # rows, columns and strides
+    l.gvk_block_quantize.restype = i32
+    l.gvk_block_quantize.argtypes = [vp, i32, vp, wide, i32, wide, vp, wide, vp]
+    l.gvk_block_dequantize.restype = i32
+    l.gvk_block_dequantize.argtypes = [vp, vp, wide, vp, wide, i32, i32, vp, wide]
+    l.gvk_block_logits_workspace.restype = C.c_size_t
+    l.gvk_block_logits_workspace.argtypes = [wide, i32]
+    l.gvk_block_logits.restype = i32
+    l.gvk_block_logits.argtypes = [vp, i32, vp, wide, wide, vp, wide, vp, wide, i32, i32, vp, wide, vp, C.c_size_t]
+    l.gvk_top_logits_workspace.restype = C.c_size_t
+    l.gvk_top_logits_workspace.argtypes = [i32, wide, wide, i32]
+    l.gvk_top_logits.restype = i32
+    l.gvk_top_logits.argtypes = [vp, i32, vp, wide, wide, wide, i32, f32, vp, vp, vp, vp, C.c_size_t]
+    l.gvk_distill_workspace.restype = C.c_size_t
+    l.gvk_distill_workspace.argtypes = [i32, wide, wide, i32]
+    l.gvk_distill.restype = i32
+    l.gvk_distill.argtypes = [vp, i32, vp, wide, wide, wide, i32, vp, vp, vp, f32, vp, vp, vp, vp, wide, vp, C.c_size_t]
+    l.gvk_distill_grad.restype = i32
+    l.gvk_distill_grad.argtypes = [vp, i32, vp, wide, wide, wide, i32, vp, vp, vp, f32, vp, vp, vp, wide]
     l.gvk_probe_row_traffic.restype = i32
     l.gvk_probe_row_traffic.argtypes = [vp, i32, vp, vp, vp, vp, C.c_float, i32]
     l.gvk_alias_sample.restype = i32

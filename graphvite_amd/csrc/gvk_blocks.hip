@@ -1,0 +1,442 @@
+// Logits of query rows against a whole table of candidates held in 8 bits: gvk_block_quantize, gvk_block_dequantize,
+// gvk_block_logits (include/gvk.h).
+//
+//   table      x[n][c] = value[n][c] * 2^(exponent[n][c / 128] - 127),  value in e4m3 (one byte), exponent one byte per block of
+//              128 columns of a row: the least power of two that brings the block's largest magnitude to 448 or below.  A power of
+//              two costs e4m3 nothing (its relative step is the same at every scale) and multiplies exactly.
+//   logits     z[m][n] = sum_c q[m][c] * x[n][c],  q quantised by the same rule on the way in.
+//
+// Which matrix instruction: every e4m3 value times its power of two is a bf16 number, exactly, and the product of two of them
+// is a float, exactly; the bf16 instruction adds those with an error of float sums (measured: 1.4e-8 of the result's norm
+// over 128 columns).  The 8-bit instructions, with or without scales, align the products of a step to its largest one and
+// drop what lies below: 1.5e-5 of the norm on normal rows, 5e-5 on rows that use e4m3's whole range (measured, all four
+// shapes alike).  That is a sum in fewer than 32 bits, so the table is read in 8 bits, widened in registers by
+// v_cvt_scalef32_pk_bf16_fp8 (two values an instruction, the scale applied in it) and multiplied in bf16.
+#include <hip/hip_fp16.h>
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "gvk.h"
+#include "gvk_internal.h"
+#include "gvk_rows.hpp"
+
+namespace {
+
+using gvk_rows::from_float;
+using gvk_rows::to_float;
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kBlockColumns = 128;
+
+// exponent byte of a block from the bits of its largest magnitude (448 = 1.75 * 2^8); 255 marks a block that holds NaN or infinity
+__device__ __forceinline__ uint32_t exponent_of(uint32_t largest) {
+    if (largest >= 0x7f800000u) return 255;
+    if (largest == 0) return 127;
+    const int e = (int)(largest >> 23) - 8 + ((largest & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return (uint32_t)max(e, 0);
+}
+
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// the largest of a half wave (32 lanes: one block of columns, four to a lane)
+__device__ __forceinline__ uint32_t half_wave_max(uint32_t v) {
+#pragma unroll
+    for (int step = 1; step < 32; step <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, step));
+    return v;
+}
+
+// four e4m3 bytes of x * 2^(127 - exponent), rounded to nearest even; NaN bytes where the block is marked
+__device__ __forceinline__ uint32_t quantise4(const float x[4], uint32_t exponent) {
+    if (exponent == 255) return 0x7f7f7f7fu;
+    const int shift = 127 - (int)exponent;
+    int packed = __builtin_amdgcn_cvt_pk_fp8_f32(ldexpf(x[0], shift), ldexpf(x[1], shift), 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(ldexpf(x[2], shift), ldexpf(x[3], shift), packed, true);
+}
+
+// columns [column, column + 4) of a row as floats, zero behind its end
+template<class T>
+__device__ __forceinline__ void load4(const T *row, int column, int dim, bool wide, float out[4]) {
+    if (wide && column + 4 <= dim) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 v = *reinterpret_cast<const float4 *>(row + column);
+            out[0] = v.x, out[1] = v.y, out[2] = v.z, out[3] = v.w;
+        } else {
+            const uint2 v = *reinterpret_cast<const uint2 *>(row + column);
+            const T *t = reinterpret_cast<const T *>(&v);
+#pragma unroll
+            for (int i = 0; i < 4; i++) out[i] = to_float(t[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) out[i] = column + i < dim ? to_float(row[column + i]) : 0.0f;
+    }
+}
+
+// One half wave per (row, block): every value is read and written once, HBM bound.
+template<class T>
+__global__ void __launch_bounds__(256) quantize_kernel(const T *rows, int64_t row_stride, bool wide, uint32_t num_row, int dim, int blocks,
+                                                       int padded, uint8_t *values, int64_t value_stride, uint8_t *exponents) {
+    for (uint64_t item = (uint64_t)blockIdx.x * 8 + threadIdx.x / 32; item < (uint64_t)num_row * blocks; item += (uint64_t)gridDim.x * 8) {
+        const uint32_t row = (uint32_t)(item / blocks), block = (uint32_t)(item % blocks);
+        const int column = (int)block * kBlockColumns + (threadIdx.x & 31) * 4;
+        float x[4];
+        load4(rows + (int64_t)row * row_stride, column, dim, wide, x);
+        const uint32_t exponent = exponent_of(half_wave_max(max(max(magnitude(x[0]), magnitude(x[1])), max(magnitude(x[2]), magnitude(x[3])))));
+        if (column < padded) *reinterpret_cast<uint32_t *>(values + (int64_t)row * value_stride + column) = quantise4(x, exponent);
+        if ((threadIdx.x & 31) == 0) exponents[item] = (uint8_t)exponent;
+    }
+}
+
+template<class T>
+__global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t *values, int64_t value_stride, const uint8_t *exponents, uint32_t num_row,
+                                                         int dim, int blocks, T *rows, int64_t row_stride, bool wide) {
+    for (uint64_t item = (uint64_t)blockIdx.x * 8 + threadIdx.x / 32; item < (uint64_t)num_row * blocks; item += (uint64_t)gridDim.x * 8) {
+        const uint32_t row = (uint32_t)(item / blocks), block = (uint32_t)(item % blocks);
+        const int column = (int)block * kBlockColumns + (threadIdx.x & 31) * 4;
+        if (column >= dim) continue;
+        const int packed = *reinterpret_cast<const int *>(values + (int64_t)row * value_stride + column);  // padded to 16 columns
+        const int shift = (int)exponents[item] - 127;
+        const float x[4] = {ldexpf(__builtin_amdgcn_cvt_f32_fp8(packed, 0), shift), ldexpf(__builtin_amdgcn_cvt_f32_fp8(packed, 1), shift),
+                            ldexpf(__builtin_amdgcn_cvt_f32_fp8(packed, 2), shift), ldexpf(__builtin_amdgcn_cvt_f32_fp8(packed, 3), shift)};
+        T *out = rows + (int64_t)row * row_stride + column;
+        if (wide && column + 4 <= dim) {
+            T t[4] = {from_float<T>(x[0]), from_float<T>(x[1]), from_float<T>(x[2]), from_float<T>(x[3])};
+            if constexpr (sizeof(T) == 4)
+                *reinterpret_cast<float4 *>(out) = *reinterpret_cast<const float4 *>(t);
+            else
+                *reinterpret_cast<uint2 *>(out) = *reinterpret_cast<const uint2 *>(t);
+        } else {
+            for (int i = 0; i < 4 && column + i < dim; i++) out[i] = from_float<T>(x[i]);
+        }
+    }
+}
+
+// ---- the product ------------------------------------------------------------------------------------------------------------
+// v_mfma_f32_16x16x32_bf16 with the TABLE as its first operand: a lane then ends with four consecutive candidates of one query
+// (n = 4 * (lane / 16) + r, m = lane % 16) and stores them at once.
+// Inside a block of 128 columns the order of the columns is free as long as both operands agree.  Lane group g = lane / 16 takes
+// columns j * 64 + g * 16 .. + 16 for j = 0, 1 — sixteen consecutive bytes of a table row, one load — and step s = 2 j + h of
+// the four 32-column steps multiplies the half h of them.
+// Queries are laid out once as the fragments of that order: [block][16-row tile][step][lane][8] bf16, 4 KB per tile and block,
+// so that a wave reads a fragment as one contiguous KB, from LDS without bank conflicts.
+
+constexpr int kFragment = 512;  // bf16 numbers of a (tile, block, step)
+
+// the place of query column c (inside its block) of row m (inside its tile)
+__device__ __forceinline__ int fragment_place(int m, int c) {
+    const int j = c >> 6, g = (c >> 4) & 3, h = (c >> 3) & 1;
+    return (2 * j + h) * kFragment + (g * 16 + m) * 8 + (c & 7);
+}
+
+// the four columns x of query row m, quantised, as bf16 fragments (every e4m3 value times its power of two is a bf16 number)
+__device__ __forceinline__ void put_fragment(__bf16 *tile, int m, int c, const float x[4]) {
+    const uint32_t exponent = exponent_of(half_wave_max(max(max(magnitude(x[0]), magnitude(x[1])), max(magnitude(x[2]), magnitude(x[3])))));
+    const uint32_t packed = quantise4(x, exponent);
+    const float scale = __uint_as_float(exponent << 23);
+    const bf16x2 low = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(packed, scale, false);
+    const bf16x2 high = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(packed, scale, true);
+    uint2 both = {__builtin_bit_cast(uint32_t, low), __builtin_bit_cast(uint32_t, high)};
+    *reinterpret_cast<uint2 *>(tile + fragment_place(m, c)) = both;
+}
+
+// queries -> fragments [blocks][tiles][4][64][8]; rows behind the last one are zero
+template<class T>
+__global__ void __launch_bounds__(256) fragment_kernel(const T *query, int64_t query_stride, bool wide, uint32_t num_query, uint32_t tiles, int dim,
+                                                       int blocks, __bf16 *fragments) {
+    const uint32_t item = blockIdx.x * 8 + threadIdx.x / 32;  // (row, block)
+    const uint32_t row = item / blocks, block = item % blocks;
+    if (row >= tiles * 16) return;
+    const int c = (threadIdx.x & 31) * 4;
+    float x[4] = {0, 0, 0, 0};
+    if (row < num_query) load4(query + (int64_t)row * query_stride, (int)block * kBlockColumns + c, dim, wide, x);
+    put_fragment(fragments + ((size_t)block * tiles + row / 16) * 4 * kFragment, row % 16, c, x);
+}
+
+// sixteen bytes of a table row -> the two bf16 operands of steps 2 j and 2 j + 1
+__device__ __forceinline__ void widen(const uint4 raw, float scale, bf16x8 out[2]) {
+    const uint32_t word[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const bf16x2 low = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word[2 * h + i], scale, false);
+            const bf16x2 high = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word[2 * h + i], scale, true);
+            out[h][4 * i] = low[0], out[h][4 * i + 1] = low[1], out[h][4 * i + 2] = high[0], out[h][4 * i + 3] = high[1];
+        }
+    }
+}
+
+// logits [m][n .. n + 4) of one lane
+template<class T>
+__device__ __forceinline__ void store4(T *row, uint32_t n, uint32_t num_row, bool wide, const f32x4 z) {
+    if (wide && n + 4 <= num_row) {
+        T t[4] = {from_float<T>(z[0]), from_float<T>(z[1]), from_float<T>(z[2]), from_float<T>(z[3])};
+        if constexpr (sizeof(T) == 4)
+            *reinterpret_cast<float4 *>(row + n) = *reinterpret_cast<const float4 *>(t);
+        else
+            *reinterpret_cast<uint2 *>(row + n) = *reinterpret_cast<const uint2 *>(t);
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            if (n + r < num_row) row[n + r] = from_float<T>(z[r]);
+    }
+}
+
+struct table_view {
+    const uint8_t *values, *exponents;
+    int64_t value_stride;
+    uint32_t num_row;
+    int blocks, padded;  // padded: columns a row holds, dim rounded up to 16
+};
+
+// raw bytes and scales of TILES tiles of 16 table rows, block `block`
+template<int TILES>
+__device__ __forceinline__ void load_table(const table_view &t, uint32_t first, int block, uint4 raw[TILES][2], float scale[TILES]) {
+    const int lane = threadIdx.x & 63, column = block * kBlockColumns + (lane >> 4) * 16;
+#pragma unroll
+    for (int i = 0; i < TILES; i++) {
+        const uint32_t row = min(first + i * 16 + (lane & 15), t.num_row - 1);  // rows behind the last one: read, never stored
+        const uint8_t *at = t.values + (int64_t)row * t.value_stride + column;
+        raw[i][0] = column < t.padded ? *reinterpret_cast<const uint4 *>(at) : uint4{0, 0, 0, 0};
+        raw[i][1] = column + 64 < t.padded ? *reinterpret_cast<const uint4 *>(at + 64) : uint4{0, 0, 0, 0};
+        scale[i] = __uint_as_float((uint32_t)t.exponents[(size_t)row * t.blocks + block] << 23);
+    }
+}
+
+// up to 16 queries: the table is read once and that bounds it.  Each workgroup lays the queries out for itself (no launch
+// before this one) and walks over strips of 64 candidates per wave.
+constexpr int kFewBlocks = 4;  // 512 columns: 16 KB of fragments
+
+template<class Q, class T>
+__global__ void __launch_bounds__(256) few_queries_kernel(const Q *query, int64_t query_stride, bool query_wide, uint32_t num_query, int dim,
+                                                          table_view table, T *logits, int64_t logit_stride, bool wide) {
+    __shared__ __bf16 fragments[kFewBlocks * 4 * kFragment];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int item = threadIdx.x / 32; item < 16 * table.blocks; item += 8) {
+        const int row = item % 16, block = item / 16, c = (threadIdx.x & 31) * 4;
+        float x[4] = {0, 0, 0, 0};
+        if (row < (int)num_query) load4(query + row * query_stride, block * kBlockColumns + c, dim, query_wide, x);
+        put_fragment(fragments + block * 4 * kFragment, row, c, x);
+    }
+    __syncthreads();
+    const uint32_t strips = (table.num_row + 63) / 64;
+    for (uint32_t strip = blockIdx.x * 4 + wave; strip < strips; strip += gridDim.x * 4) {
+        f32x4 acc[4] = {};
+        for (int block = 0; block < table.blocks; block++) {
+            uint4 raw[4][2];
+            float scale[4];
+            load_table<4>(table, strip * 64, block, raw, scale);
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                bf16x8 b[2];
+#pragma unroll
+                for (int h = 0; h < 2; h++) b[h] = *reinterpret_cast<const bf16x8 *>(fragments + (block * 4 + 2 * j + h) * kFragment + lane * 8);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    bf16x8 a[2];
+                    widen(raw[i][j], scale[i], a);
+#pragma unroll
+                    for (int h = 0; h < 2; h++) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[h], b[h], acc[i], 0, 0, 0);
+                }
+            }
+        }
+        const uint32_t m = lane & 15;
+        if (m < num_query) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) store4(logits + (int64_t)m * logit_stride, strip * 64 + i * 16 + (lane >> 4) * 4, table.num_row, wide, acc[i]);
+        }
+    }
+}
+
+// more queries: a workgroup makes 256 candidates x 16 * TILES queries, 64 candidates to a wave, the queries' fragments of a block
+// of columns in LDS.  The workgroups that share candidates are consecutive on one XCD (its L2 then serves the table's rows).
+template<int TILES, class T>
+__global__ void __launch_bounds__(256) logits_kernel(const __bf16 *fragments, uint32_t tiles, uint32_t num_query, table_view table, T *logits,
+                                                     int64_t logit_stride, bool wide) {
+    __shared__ uint4 staged[TILES * 256];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t parts = (tiles + TILES - 1) / TILES;
+    const uint32_t xcd = blockIdx.x % 8, turn = blockIdx.x / 8;
+    const uint32_t part = turn % parts, strip = (turn / parts) * 8 + xcd;
+    if ((uint64_t)strip * 256 >= table.num_row) return;  // the whole workgroup
+    const uint32_t first = strip * 256 + wave * 64, tile0 = part * TILES;
+    f32x4 acc[4][TILES] = {};
+    for (int block = 0; block < table.blocks; block++) {
+        uint4 raw[4][2];
+        float scale[4];
+        load_table<4>(table, first, block, raw, scale);
+        if (block) __syncthreads();
+        const uint4 *source = reinterpret_cast<const uint4 *>(fragments + ((size_t)block * tiles + tile0) * 4 * kFragment);
+        const uint32_t held = min((uint32_t)TILES, tiles - tile0) * 256;
+#pragma unroll
+        for (int i = 0; i < TILES; i++) staged[i * 256 + threadIdx.x] = i * 256u + threadIdx.x < held ? source[i * 256 + threadIdx.x] : uint4{0, 0, 0, 0};
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            bf16x8 a[4][2];
+#pragma unroll
+            for (int i = 0; i < 4; i++) widen(raw[i][j], scale[i], a[i]);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+#pragma unroll
+                for (int tile = 0; tile < TILES; tile++) {
+                    const bf16x8 b = __builtin_bit_cast(bf16x8, staged[(tile * 4 + 2 * j + h) * 64 + lane]);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[i][tile] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i][h], b, acc[i][tile], 0, 0, 0);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int tile = 0; tile < TILES; tile++) {
+        const uint32_t m = (tile0 + tile) * 16 + (lane & 15);
+        if (m < num_query) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) store4(logits + (int64_t)m * logit_stride, first + i * 16 + (lane >> 4) * 4, table.num_row, wide, acc[i][tile]);
+        }
+    }
+}
+
+bool aligned(const void *p, int64_t stride_bytes, size_t to) { return (uintptr_t)p % to == 0 && stride_bytes % (int64_t)to == 0; }
+
+int check_rows(const char *who, int dtype, int64_t num_row, int dim, int64_t stride) {
+    if (dtype != GVK_F32 && dtype != GVK_BF16 && dtype != GVK_F16) return gvk_fail(GVK_EINVAL, "%s: unknown type %d", who, dtype);
+    if (num_row < 0 || num_row > GVK_MAX_BLOCK_ROWS) return gvk_fail(GVK_EINVAL, "%s: %lld rows", who, (long long)num_row);
+    if (dim < 1 || dim > GVK_MAX_BLOCK_DIM) return gvk_fail(GVK_EDIM, "%s: dim must be 1 to %d, not %d", who, GVK_MAX_BLOCK_DIM, dim);
+    if (stride < dim) return gvk_fail(GVK_EINVAL, "%s: a row of %d columns with a stride of %lld", who, dim, (long long)stride);
+    return GVK_OK;
+}
+
+int check_table(const char *who, const void *values, int64_t value_stride, const void *exponents, int dim) {
+    if (!values || !exponents) return gvk_fail(GVK_EINVAL, "%s: null pointer", who);
+    if (value_stride < (dim + 15) / 16 * 16) return gvk_fail(GVK_EINVAL, "%s: %d columns need a value stride of %d, not %lld", who, dim, (dim + 15) / 16 * 16, (long long)value_stride);
+    if (!aligned(values, value_stride, 16)) return gvk_fail(GVK_EINVAL, "%s: values and their stride must be multiples of 16 bytes", who);
+    return GVK_OK;
+}
+
+dim3 item_grid(uint64_t items) {  // one half wave per item, eight to a workgroup; more items than this take turns
+    const uint64_t groups = (items + 7) / 8;
+    return dim3((unsigned)(groups < (1u << 20) ? groups : (1u << 20)));
+}
+
+int launched(const char *who) {
+    const hipError_t err = hipGetLastError();
+    return err == hipSuccess ? GVK_OK : gvk_fail(GVK_EHIP, "%s: %s", who, hipGetErrorString(err));
+}
+
+template<class Q, class T>
+int launch_logits(hipStream_t stream, const Q *query, int64_t query_stride, uint32_t num_query, int dim, const table_view &table, T *logits,
+                  int64_t logit_stride, void *workspace) {
+    const bool query_wide = aligned(query, query_stride * (int64_t)sizeof(Q), 4 * sizeof(Q));
+    const bool wide = aligned(logits, logit_stride * (int64_t)sizeof(T), 4 * sizeof(T));
+    if (!workspace) {
+        const uint32_t groups = (table.num_row + 255) / 256;
+        hipLaunchKernelGGL((few_queries_kernel<Q, T>), dim3(groups < 2048 ? groups : 2048), dim3(256), 0, stream, query, query_stride, query_wide,
+                           num_query, dim, table, logits, logit_stride, wide);
+        return launched("gvk_block_logits");
+    }
+    const uint32_t tiles = (num_query + 15) / 16;
+    __bf16 *fragments = reinterpret_cast<__bf16 *>(workspace);
+    hipLaunchKernelGGL((fragment_kernel<Q>), dim3((tiles * 16 * table.blocks + 7) / 8), dim3(256), 0, stream, query, query_stride, query_wide,
+                       num_query, tiles, dim, table.blocks, fragments);
+    const uint64_t strips = ((uint64_t)table.num_row + 255) / 256;
+#define GVK_LOGITS(TILES)                                                                                                                 \
+    {                                                                                                                                     \
+        const uint64_t grid = (strips + 7) / 8 * 8 * ((tiles + TILES - 1) / TILES);                                                       \
+        if (grid > 0xffffffull) return gvk_fail(GVK_EINVAL, "gvk_block_logits: too many logits for one call");                          \
+        hipLaunchKernelGGL((logits_kernel<TILES, T>), dim3((unsigned)grid), dim3(256), 0, stream, fragments, tiles, num_query, table, logits, \
+                           logit_stride, wide);                                                                                           \
+    }
+    if (tiles <= 1) GVK_LOGITS(1)
+    else if (tiles <= 2) GVK_LOGITS(2)
+    else if (tiles <= 4) GVK_LOGITS(4)
+    else GVK_LOGITS(8)
+#undef GVK_LOGITS
+    return launched("gvk_block_logits");
+}
+
+template<class Q>
+int launch_logits_to(hipStream_t stream, const Q *query, int64_t query_stride, uint32_t num_query, int dim, const table_view &table, int out, void *logits,
+                     int64_t logit_stride, void *workspace) {
+    switch (out) {
+        case GVK_F32: return launch_logits(stream, query, query_stride, num_query, dim, table, (float *)logits, logit_stride, workspace);
+        case GVK_BF16: return launch_logits(stream, query, query_stride, num_query, dim, table, (__bf16 *)logits, logit_stride, workspace);
+        default: return launch_logits(stream, query, query_stride, num_query, dim, table, (_Float16 *)logits, logit_stride, workspace);
+    }
+}
+
+}  // namespace
+
+extern "C" int gvk_block_quantize(void *stream, int dtype, const void *rows, int64_t num_row, int dim, int64_t row_stride, uint8_t *values,
+                                  int64_t value_stride, uint8_t *exponents) {
+    const char *who = "gvk_block_quantize";
+    int rc = check_rows(who, dtype, num_row, dim, row_stride);
+    if (rc != GVK_OK) return rc;
+    if (num_row == 0) return GVK_OK;
+    if (!rows) return gvk_fail(GVK_EINVAL, "%s: null pointer", who);
+    if ((rc = check_table(who, values, value_stride, exponents, dim)) != GVK_OK) return rc;
+    const int blocks = (dim + kBlockColumns - 1) / kBlockColumns, padded = (dim + 15) / 16 * 16;
+    const dim3 grid = item_grid((uint64_t)num_row * blocks);
+#define GVK_QUANTIZE(T)                                                                                                                    \
+    hipLaunchKernelGGL((quantize_kernel<T>), grid, dim3(256), 0, (hipStream_t)stream, (const T *)rows, row_stride,                           \
+                       aligned(rows, row_stride * (int64_t)sizeof(T), 4 * sizeof(T)), (uint32_t)num_row, dim, blocks, padded, values, value_stride, exponents)
+    if (dtype == GVK_F32) GVK_QUANTIZE(float);
+    else if (dtype == GVK_BF16) GVK_QUANTIZE(__bf16);
+    else GVK_QUANTIZE(_Float16);
+#undef GVK_QUANTIZE
+    return launched(who);
+}
+
+extern "C" int gvk_block_dequantize(void *stream, const uint8_t *values, int64_t value_stride, const uint8_t *exponents, int64_t num_row, int dim,
+                                    int dtype, void *rows, int64_t row_stride) {
+    const char *who = "gvk_block_dequantize";
+    int rc = check_rows(who, dtype, num_row, dim, row_stride);
+    if (rc != GVK_OK) return rc;
+    if (num_row == 0) return GVK_OK;
+    if (!rows) return gvk_fail(GVK_EINVAL, "%s: null pointer", who);
+    if ((rc = check_table(who, values, value_stride, exponents, dim)) != GVK_OK) return rc;
+    const int blocks = (dim + kBlockColumns - 1) / kBlockColumns;
+    const dim3 grid = item_grid((uint64_t)num_row * blocks);
+#define GVK_DEQUANTIZE(T)                                                                                                                 \
+    hipLaunchKernelGGL((dequantize_kernel<T>), grid, dim3(256), 0, (hipStream_t)stream, values, value_stride, exponents, (uint32_t)num_row, dim, blocks, \
+                       (T *)rows, row_stride, aligned(rows, row_stride * (int64_t)sizeof(T), 4 * sizeof(T)))
+    if (dtype == GVK_F32) GVK_DEQUANTIZE(float);
+    else if (dtype == GVK_BF16) GVK_DEQUANTIZE(__bf16);
+    else GVK_DEQUANTIZE(_Float16);
+#undef GVK_DEQUANTIZE
+    return launched(who);
+}
+
+extern "C" size_t gvk_block_logits_workspace(int64_t num_query, int dim) {
+    const int64_t blocks = (dim + kBlockColumns - 1) / kBlockColumns;
+    if (num_query < 1 || dim < 1 || (num_query <= 16 && blocks <= kFewBlocks)) return 0;
+    return (size_t)((num_query + 15) / 16 * blocks) * 4 * kFragment * sizeof(__bf16);
+}
+
+extern "C" int gvk_block_logits(void *stream, int query_dtype, const void *query, int64_t num_query, int64_t query_stride, const uint8_t *values,
+                                int64_t value_stride, const uint8_t *exponents, int64_t num_row, int dim, int logit_dtype, void *logits,
+                                int64_t logit_stride, void *workspace, size_t workspace_bytes) {
+    const char *who = "gvk_block_logits";
+    int rc = check_rows(who, query_dtype, num_query, dim, query_stride);
+    if (rc != GVK_OK) return rc;
+    if (num_query > GVK_MAX_BLOCK_QUERIES) return gvk_fail(GVK_EINVAL, "%s: %lld queries; a call takes %d", who, (long long)num_query, GVK_MAX_BLOCK_QUERIES);
+    if (logit_dtype != GVK_F32 && logit_dtype != GVK_BF16 && logit_dtype != GVK_F16) return gvk_fail(GVK_EINVAL, "%s: unknown type %d", who, logit_dtype);
+    if (num_row < 0 || num_row > GVK_MAX_BLOCK_ROWS) return gvk_fail(GVK_EINVAL, "%s: %lld rows", who, (long long)num_row);
+    if (logit_stride < num_row) return gvk_fail(GVK_EINVAL, "%s: rows of %lld logits with a stride of %lld", who, (long long)num_row, (long long)logit_stride);
+    if (num_query == 0 || num_row == 0) return GVK_OK;
+    if (!query || !logits) return gvk_fail(GVK_EINVAL, "%s: null pointer", who);
+    if ((rc = check_table(who, values, value_stride, exponents, dim)) != GVK_OK) return rc;
+    const size_t need = gvk_block_logits_workspace(num_query, dim);
+    if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
+        return gvk_fail(GVK_EINVAL, "%s: needs a workspace of %zu bytes on a multiple of 16, %zu given", who, need, workspace ? workspace_bytes : (size_t)0);
+    const table_view table = {values, exponents, value_stride, (uint32_t)num_row, (dim + kBlockColumns - 1) / kBlockColumns, (dim + 15) / 16 * 16};
+    void *const space = need ? workspace : nullptr;
+    switch (query_dtype) {
+        case GVK_F32: return launch_logits_to((hipStream_t)stream, (const float *)query, query_stride, (uint32_t)num_query, dim, table, logit_dtype, logits, logit_stride, space);
+        case GVK_BF16: return launch_logits_to((hipStream_t)stream, (const __bf16 *)query, query_stride, (uint32_t)num_query, dim, table, logit_dtype, logits, logit_stride, space);
+        default: return launch_logits_to((hipStream_t)stream, (const _Float16 *)query, query_stride, (uint32_t)num_query, dim, table, logit_dtype, logits, logit_stride, space);
+    }
+}

@@ -1,0 +1,101 @@
+// Device code shared by the kernels over whole rows of logits or embeddings (gvk_blocks.hip, gvk_logits.hip): the three
+// element types, a row seen as aligned 16-byte chunks, reductions over a workgroup.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace gvk_rows {
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__bf16 x) { return (float)x; }
+__device__ __forceinline__ float to_float(_Float16 x) { return (float)x; }
+
+// rounded once, to nearest even
+template<class T>
+__device__ __forceinline__ T from_float(float x) { return (T)x; }
+
+template<class T>
+struct per_chunk {
+    static constexpr int value = 16 / (int)sizeof(T);
+};
+
+// A row of n elements as chunks of 16 bytes on multiples of 16 bytes: chunk c holds elements c * E - lead ... + E, those in
+// front of the row and behind it read as minus infinity.  Rows may start anywhere (an odd stride of 16-bit numbers): only
+// the first and the last chunk are read element by element, nothing outside the row is touched.
+template<class T>
+struct chunked_row {
+    static constexpr int E = per_chunk<T>::value;
+    const T *row;
+    int64_t n;
+    int lead;
+
+    __device__ __forceinline__ chunked_row(const T *row, int64_t n) : row(row), n(n), lead((int)((uintptr_t)row % 16 / sizeof(T))) {}
+    __device__ __forceinline__ int64_t chunks() const { return (n + lead + E - 1) / E; }
+    __device__ __forceinline__ int64_t first(int64_t chunk) const { return chunk * E - lead; }
+    __device__ __forceinline__ uint4 load(int64_t chunk) const {
+        const int64_t at = first(chunk);
+        if (at >= 0 && at + E <= n) return *reinterpret_cast<const uint4 *>(row + at);
+        uint4 raw;
+        T t[E];
+#pragma unroll
+        for (int i = 0; i < E; i++) t[i] = at + i >= 0 && at + i < n ? row[at + i] : (T)(-__builtin_inff());
+        __builtin_memcpy(&raw, t, 16);
+        return raw;
+    }
+};
+
+template<class T>
+__device__ __forceinline__ void unpack(const uint4 raw, float x[per_chunk<T>::value]) {
+    T t[per_chunk<T>::value];
+    __builtin_memcpy(t, &raw, 16);
+#pragma unroll
+    for (int i = 0; i < per_chunk<T>::value; i++) x[i] = to_float(t[i]);
+}
+
+// chunk `at` (its first element's index) of a row of n elements <- x; the row shares its lead with the row that x came from
+// where `wide`, else every element is stored by itself
+template<class T>
+__device__ __forceinline__ void store_chunk(T *row, int64_t at, int64_t n, bool wide, const float x[per_chunk<T>::value]) {
+    constexpr int E = per_chunk<T>::value;
+    T t[E];
+#pragma unroll
+    for (int i = 0; i < E; i++) t[i] = from_float<T>(x[i]);
+    if (wide && at >= 0 && at + E <= n) {
+        uint4 raw;
+        __builtin_memcpy(&raw, t, 16);
+        *reinterpret_cast<uint4 *>(row + at) = raw;
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; i++)
+            if (at + i >= 0 && at + i < n) row[at + i] = t[i];
+    }
+}
+
+// max / sum over a workgroup of THREADS threads, every thread gets it; `shared` holds THREADS / 64 floats.  Fixed order.
+template<int THREADS>
+__device__ __forceinline__ float block_max(float v, float *shared) {
+#pragma unroll
+    for (int step = 1; step < 64; step <<= 1) v = fmaxf(v, __shfl_xor(v, step));
+    __syncthreads();  // the last use of `shared` is over
+    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = shared[0];
+#pragma unroll
+    for (int i = 1; i < THREADS / 64; i++) v = fmaxf(v, shared[i]);
+    return v;
+}
+
+template<int THREADS>
+__device__ __forceinline__ float block_sum(float v, float *shared) {
+#pragma unroll
+    for (int step = 1; step < 64; step <<= 1) v += __shfl_xor(v, step);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = shared[0];
+#pragma unroll
+    for (int i = 1; i < THREADS / 64; i++) v += shared[i];
+    return v;
+}
+
+}  // namespace gvk_rows

@@ -88,6 +88,94 @@ class OptimizerSpec(object):
                               self.hp1, self.epsilon)
 
 
+_ROW_TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+def _need_rows(t, name, device=None, dtypes=_ROW_TYPES, shape=None):
+    """A 2-D GPU tensor whose rows are contiguous (any row stride that keeps them apart)."""
+    if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.dim() != 2:
+        raise ValueError("%s must be a two-dimensional torch tensor of dtype %s" % (name, " or ".join(str(d) for d in dtypes)))
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError("%s has shape %s, expected %s" % (name, tuple(t.shape), tuple(shape)))
+    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise ValueError("the rows of %s must be contiguous and must not overlap (strides %s)" % (name, t.stride()))
+    if device is not None and t.device != device:
+        raise ValueError("%s lives on %s, expected %s" % (name, t.device, device))
+    if not t.is_cuda:
+        raise ValueError("%s must live in GPU memory; graphvite_amd has no CPU path for it" % name)
+    return t
+
+
+def _row_stride(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _need_shape(t, dtype, name, device, shape):
+    _need(t, dtype, name, device)
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError("%s has shape %s, expected %s" % (name, tuple(t.shape), tuple(shape)))
+    return t
+
+
+class BlockTable(object):
+    """A table of rows in 8 bits with a power-of-two scale for each block of 128 columns of a row (include/gvk.h,
+    gvk_block_quantize): row r, column c stands for e4m3(values[r, c]) * 2 ** (exponents[r, c // 128] - 127).
+
+    Parameters:
+        values (Tensor): uint8 or float8_e4m3fn [rows, >= dim rounded up to 16], a row stride of a multiple of 16 bytes; the
+            columns between dim and that multiple are zero
+        exponents (Tensor): uint8 [rows, (dim + 127) // 128]
+        dim (int): columns of a row, 1 to 4096
+
+    HipKernels.quantize_blocks makes one; a quarter of the bytes of the float32 rows.
+    """
+
+    def __init__(self, values, exponents, dim):
+        dim = int(dim)
+        if not 1 <= dim <= _lib.MAX_BLOCK_DIM:
+            raise ValueError("dim must be 1 to %d, not %d" % (_lib.MAX_BLOCK_DIM, dim))
+        _need_rows(values, "values", None, (torch.uint8, torch.float8_e4m3fn))
+        _need_shape(exponents, torch.uint8, "exponents", values.device, (values.shape[0], (dim + 127) // 128))
+        if values.shape[1] < (dim + 15) // 16 * 16 or values.data_ptr() % 16 or values.shape[0] > 1 and values.stride(0) % 16:
+            raise ValueError("values must hold dim rounded up to 16 columns per row, and start and step by multiples of 16 bytes")
+        self.values, self.exponents, self.dim = values, exponents, dim
+
+    @staticmethod
+    def empty(rows, dim, device):
+        """An uninitialised table for HipKernels.quantize_blocks to fill."""
+        return BlockTable(torch.empty((rows, (int(dim) + 15) // 16 * 16), dtype=torch.uint8, device=device),
+                          torch.empty((rows, (int(dim) + 127) // 128), dtype=torch.uint8, device=device), dim)
+
+    @property
+    def rows(self):
+        return self.values.shape[0]
+
+    @property
+    def device(self):
+        return self.values.device
+
+    @property
+    def _stride(self):
+        return self.values.stride(0) if self.rows > 1 else self.values.shape[1] // 16 * 16
+
+
+class _on(object):
+    """Launches go to the tensors' device, whichever is current."""
+
+    def __init__(self, device):
+        self.device = device
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.device.index:
+            torch.cuda.set_device(self.device)
+
+    def __exit__(self, *exc):
+        if self.before != self.device.index:
+            torch.cuda.set_device(self.before)
+        return False
+
+
 class HipKernels(object):
     """Launches on torch's current stream of the tensors' device."""
 
@@ -263,6 +351,124 @@ class HipKernels(object):
         rc = self.lib.gvk_predict(self._stream(vertex), vertex.shape[1], _ptr(vertex), _ptr(context), _ptr(pairs),
                                   _ptr(logits), pairs.shape[0])
         _lib.check(rc, "gvk_predict")
+
+    # ------------------------------------------------------------------------------------------- whole rows of candidates
+    @staticmethod
+    def _workspace(nbytes, device):
+        """Scratch of one call: torch's allocator hands it on once the current stream has passed the call (a captured graph
+        has its own)."""
+        return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+    def quantize_blocks(self, rows, table=None):
+        """Rows (float32, bfloat16 or float16 [n, dim]) -> BlockTable: e4m3 with a power-of-two scale per 128 columns of a
+        row.  `table`: an existing one of that shape to overwrite."""
+        _need_rows(rows, "rows")
+        if table is None:
+            table = BlockTable.empty(rows.shape[0], rows.shape[1], rows.device)
+        if not isinstance(table, BlockTable) or table.device != rows.device or (table.rows, table.dim) != tuple(rows.shape):
+            raise ValueError("table must be a BlockTable of the rows' shape on their device")
+        with _on(rows.device):
+            rc = self.lib.gvk_block_quantize(self._stream(rows), _ROW_TYPES[rows.dtype], _ptr(rows), rows.shape[0], rows.shape[1],
+                                             _row_stride(rows), _ptr(table.values), table._stride, _ptr(table.exponents))
+        _lib.check(rc, "gvk_block_quantize")
+        return table
+
+    def dequantize_blocks(self, table, rows):
+        """BlockTable -> rows (float32, bfloat16 or float16 [n, dim])."""
+        _need_rows(rows, "rows", table.device, shape=(table.rows, table.dim))
+        with _on(rows.device):
+            rc = self.lib.gvk_block_dequantize(self._stream(rows), _ptr(table.values), table._stride, _ptr(table.exponents), table.rows,
+                                               table.dim, _ROW_TYPES[rows.dtype], _ptr(rows), _row_stride(rows))
+        _lib.check(rc, "gvk_block_dequantize")
+        return rows
+
+    def block_logits(self, query, table, logits):
+        """logits[m, n] = <query[m] quantised to 8 bits, table[n]>: every query against every row of a BlockTable, in float32,
+        bfloat16 or float16.  Queries are quantised on the way in (blocks of 128 columns, as quantize_blocks)."""
+        if not isinstance(table, BlockTable):
+            raise ValueError("table must be a BlockTable")
+        dev = table.device
+        _need_rows(query, "query", dev)
+        _need_rows(logits, "logits", dev, shape=(query.shape[0], table.rows))
+        if query.shape[1] != table.dim:
+            raise ValueError("queries of %d columns against a table of %d" % (query.shape[1], table.dim))
+        nbytes = self.lib.gvk_block_logits_workspace(query.shape[0], table.dim)
+        with _on(dev):
+            workspace = self._workspace(nbytes, dev)
+            rc = self.lib.gvk_block_logits(self._stream(logits), _ROW_TYPES[query.dtype], _ptr(query), query.shape[0], _row_stride(query),
+                                           _ptr(table.values), table._stride, _ptr(table.exponents), table.rows, table.dim,
+                                           _ROW_TYPES[logits.dtype], _ptr(logits), _row_stride(logits), _ptr(workspace), nbytes)
+        _lib.check(rc, "gvk_block_logits")
+        return logits
+
+    def top_logits(self, logits, values, index, stats=None, temperature=1.0):
+        """The k = values.shape[1] largest logits of each row: values float32 [m, k], largest first, of equal ones the lowest
+        candidate; index int32 [m, k]; stats float32 [m, 2] = {max, log sum exp((logit - max) / temperature)}."""
+        dev = logits.device if isinstance(logits, torch.Tensor) else None
+        _need_rows(logits, "logits")
+        if not isinstance(values, torch.Tensor) or values.dim() != 2:
+            raise ValueError("values must be [rows, k]")
+        rows, k = logits.shape[0], values.shape[1]
+        _need_shape(values, torch.float32, "values", dev, (rows, k))
+        _need_shape(index, torch.int32, "index", dev, (rows, k))
+        if stats is not None:
+            _need_shape(stats, torch.float32, "stats", dev, (rows, 2))
+        dtype = _ROW_TYPES[logits.dtype]
+        nbytes = self.lib.gvk_top_logits_workspace(dtype, rows, logits.shape[1], k)
+        with _on(dev):
+            workspace = self._workspace(nbytes, dev)
+            rc = self.lib.gvk_top_logits(self._stream(logits), dtype, _ptr(logits), rows, logits.shape[1], _row_stride(logits), k,
+                                         temperature, _ptr(values), _ptr(index), _ptr(stats), _ptr(workspace), nbytes)
+        _lib.check(rc, "gvk_top_logits")
+        return values, index
+
+    @staticmethod
+    def _distill_list(logits, index, teacher, teacher_stats, weight):
+        _need_rows(logits, "logits")
+        dev, rows = logits.device, logits.shape[0]
+        if not isinstance(index, torch.Tensor) or index.dim() != 2:
+            raise ValueError("index must be [rows, k]")
+        _need_shape(index, torch.int32, "index", dev, (rows, index.shape[1]))
+        _need_shape(teacher, torch.float32, "teacher", dev, index.shape)
+        if teacher_stats is not None:
+            _need_shape(teacher_stats, torch.float32, "teacher_stats", dev, (rows, 2))
+        if weight is not None:
+            _need_shape(weight, torch.float32, "weight", dev, (rows,))
+        return dev, rows, index.shape[1]
+
+    def distill(self, logits, index, teacher, loss, stats, teacher_stats=None, temperature=1.0, weight=None, grad=None):
+        """Kullback-Leibler divergence of softmax(logits / temperature) from a teacher's top logits, per row, and — with `grad` —
+        its gradient by the logits, weighted by weight[row] (the derivative by the row's loss; 1 without).
+
+        index int32 [m, k]: candidates of the teacher's list (-1: no entry); teacher float32 [m, k]: their logits; teacher_stats
+        float32 [m, 2] (top_logits of the teacher at the same temperature): probabilities of the teacher's whole row instead of the
+        list's own; loss float32 [m], stats float32 [m, 2] are written; grad: like logits, may be logits itself."""
+        dev, rows, k = self._distill_list(logits, index, teacher, teacher_stats, weight)
+        _need_shape(loss, torch.float32, "loss", dev, (rows,))
+        _need_shape(stats, torch.float32, "stats", dev, (rows, 2))
+        if grad is not None:
+            _need_rows(grad, "grad", dev, (logits.dtype,), logits.shape)
+        dtype = _ROW_TYPES[logits.dtype]
+        nbytes = self.lib.gvk_distill_workspace(dtype, rows, logits.shape[1], k)
+        with _on(dev):
+            workspace = self._workspace(nbytes, dev)
+            rc = self.lib.gvk_distill(self._stream(logits), dtype, _ptr(logits), rows, logits.shape[1], _row_stride(logits), k, _ptr(index),
+                                      _ptr(teacher), _ptr(teacher_stats), temperature, _ptr(weight), _ptr(loss), _ptr(stats), _ptr(grad),
+                                      0 if grad is None else _row_stride(grad), _ptr(workspace), nbytes)
+        _lib.check(rc, "gvk_distill")
+        return loss
+
+    def distill_grad(self, logits, index, teacher, stats, grad, teacher_stats=None, temperature=1.0, weight=None):
+        """The gradient of distill alone, from the stats that a forward pass over the same logits wrote."""
+        dev, rows, k = self._distill_list(logits, index, teacher, teacher_stats, weight)
+        _need_shape(stats, torch.float32, "stats", dev, (rows, 2))
+        _need_rows(grad, "grad", dev, (logits.dtype,), logits.shape)
+        with _on(dev):
+            rc = self.lib.gvk_distill_grad(self._stream(logits), _ROW_TYPES[logits.dtype], _ptr(logits), rows, logits.shape[1],
+                                           _row_stride(logits), k, _ptr(index), _ptr(teacher), _ptr(teacher_stats), temperature,
+                                           _ptr(weight), _ptr(stats), _ptr(grad), _row_stride(grad))
+        _lib.check(rc, "gvk_distill_grad")
+        return grad
 
     def probe_row_traffic(self, vertex, context, pairs, negatives, bump=0.0):
         """Measurement aid (gvk_probe_row_traffic): read and write back the head, tail and given negative row of every

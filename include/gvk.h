@@ -433,6 +433,70 @@ int gvk_has_ab_builds(void);
 int gvk_describe_train(int dim, int optimizer_type, int num_negative, int explicit_negatives, int batch_size,
                        uint32_t n_vertex, char *name, size_t capacity);
 
+/* ---- whole rows: logits of every candidate, the best of them, learning from them ------------------------------------------
+ * gvk_predict answers for given pairs; these answer for a node against every candidate.  No counterpart in the reference's
+ * node-embedding path (its knowledge-graph application ranks all entities by predicting every pair,
+ * python/graphvite/application/application.py:759-847).
+ *
+ * Element types of rows, queries, logits and gradients. */
+enum { GVK_F32 = 0, GVK_BF16 = 1, GVK_F16 = 2 };
+#define GVK_MAX_BLOCK_DIM 4096
+#define GVK_MAX_BLOCK_ROWS 0x7fffff00
+#define GVK_MAX_BLOCK_QUERIES (1 << 20)
+#define GVK_MAX_TOP 256            /* entries gvk_top_logits gives per row */
+#define GVK_MAX_DISTILL_LIST 1024  /* entries of a teacher's list */
+
+/* A table of rows in 8 bits:  x[r][c] = value[r][c] * 2^(exponent[r][c / 128] - 127).
+ *   values     one e4m3 byte per column (largest magnitude 448, no infinity, 0x7f = NaN); value_stride bytes from row to row, both it and
+ *              the pointer multiples of 16; columns dim ... up to a multiple of 16 are part of a row and hold zero
+ *   exponents  one byte per block of 128 columns, [num_row][(dim + 127) / 128]: the least with max |x| <= 448 * 2^(exponent - 127), 127
+ *              for a block of zeros, 0 at the least (below 2^-118 or so values round to e4m3's least steps of it);
+ *              255 marks a block that held a NaN or an infinity: all of it reads as NaN
+ * Values round to nearest, ties to even: off by at most 2^-4 of a value, or 2^-10 * 2^(exponent - 127) for the least ones.
+ * num_row up to GVK_MAX_BLOCK_ROWS, dim 1 ... GVK_MAX_BLOCK_DIM, row_stride >= dim elements; rows may have any alignment of their type. */
+int gvk_block_quantize(void *stream, int dtype, const void *rows, int64_t num_row, int dim, int64_t row_stride, uint8_t *values, int64_t value_stride,
+                       uint8_t *exponents);
+/* the table as numbers, each rounded once to `dtype` */
+int gvk_block_dequantize(void *stream, const uint8_t *values, int64_t value_stride, const uint8_t *exponents, int64_t num_row, int dim, int dtype, void *rows,
+                         int64_t row_stride);
+/* logits[m][n] = sum_c q[m][c] * x[n][c]: q = the queries quantised as gvk_block_quantize does, sums in 32 bits, each logit rounded
+ * once to `logit_dtype`.  (Products count bf16 numbers below 2^-126 as zero.)  logit_stride >= num_row elements; nothing between
+ * a row's end and the next row is written.  The workspace (gvk_block_logits_workspace bytes, on a multiple of 16; none for up to 16 queries
+ * of up to 512 columns) belongs to the call until the stream has passed it.  Same inputs, same bits. */
+size_t gvk_block_logits_workspace(int64_t num_query, int dim);
+int gvk_block_logits(void *stream, int query_dtype, const void *query, int64_t num_query, int64_t query_stride, const uint8_t *values, int64_t value_stride,
+                     const uint8_t *exponents, int64_t num_row, int dim, int logit_dtype, void *logits, int64_t logit_stride, void *workspace,
+                     size_t workspace_bytes);
+
+/* The k largest logits of each row, largest first, of equal ones the lowest candidate: values[r][0 .. k) (as floats, exactly; -0 as 0),
+ * index[r][0 .. k).  NaN counts as the largest.  Minus infinity is a logit like others (a masked candidate; it comes last).
+ * stats[r] = {m, log sum_j exp((z_j - m) / temperature)}, m = max_j z_j, or null; {-inf, -inf} where every logit is minus infinity, NaN in the
+ * second place where a logit is NaN or plus infinity.  1 <= k <= min(num_col, GVK_MAX_TOP).  Workspace as above. */
+size_t gvk_top_logits_workspace(int dtype, int64_t num_row, int64_t num_col, int k);
+int gvk_top_logits(void *stream, int dtype, const void *logits, int64_t num_row, int64_t num_col, int64_t stride, int k, float temperature, float *values,
+                   int32_t *index, float *stats, void *workspace, size_t workspace_bytes);
+
+/* Distillation from a teacher's top logits.  Row r of the student's logits z (num_col candidates, minus infinity = masked) against a list of
+ * k entries, index[r][e] (a candidate, or -1: no entry) and teacher[r][e] (its logit; minus infinity: no entry):
+ *     p_j = exp((z_j - m) / temperature) / S                 over all candidates
+ *     q_e = exp((t_e - mt) / temperature) / St               mt, St: of the list; with teacher_stats = {mt, log St} of the teacher's whole
+ *                                                            row (gvk_top_logits at the same temperature), and Q = sum q_e is below 1
+ *     loss[r]    = sum_e q_e (log q_e - log p_{index e})      (unweighted)
+ *     stats[r]   = {m, log S}                                  what gvk_distill_grad takes
+ *     grad[r][j] = weight[r] / temperature * (Q p_j - sum_{e: index e = j} q_e)       weight null: 1
+ * `weight` is the derivative by loss[r].  A candidate may be listed more than once: its entries add.  A row without entries, or with every
+ * candidate masked, has loss and gradient 0.  A listed candidate that is masked makes the loss infinite.  An index below -1 or not
+ * below num_col makes the row's loss and gradient NaN.  grad has the logits' type, is rounded once, and may be the logits themselves
+ * (same pointer and stride); null: the loss alone.  Same inputs, rows beginning alike within 16 bytes: same bits.  1 <= k <= GVK_MAX_DISTILL_LIST. */
+size_t gvk_distill_workspace(int dtype, int64_t num_row, int64_t num_col, int k);
+int gvk_distill(void *stream, int dtype, const void *logits, int64_t num_row, int64_t num_col, int64_t stride, int k, const int32_t *index, const float *teacher,
+                const float *teacher_stats, float temperature, const float *weight, float *loss, float *stats, void *grad, int64_t grad_stride,
+                void *workspace, size_t workspace_bytes);
+/* the gradient alone, from the stats of a forward pass over the same logits */
+int gvk_distill_grad(void *stream, int dtype, const void *logits, int64_t num_row, int64_t num_col, int64_t stride, int k, const int32_t *index,
+                     const float *teacher, const float *teacher_stats, float temperature, const float *weight, const float *stats, void *grad,
+                     int64_t grad_stride);
+
 /* Named host ranges for profilers (roctx; `rocprofv3 --marker-trace`): the scopes the reference times with its
  * USE_TIMER Timer (include/util/time.h:28-60, include/core/solver.h:622,645,1526-1552).  Nesting allowed, per thread. */
 void gvk_range_push(const char *name);
