@@ -142,17 +142,31 @@ __device__ __forceinline__ void put_fragment(__bf16 *tile, int m, int c, const f
     *reinterpret_cast<uint2 *>(tile + fragment_place(m, c)) = both;
 }
 
-// queries -> fragments [blocks][tiles][4][64][8]; rows behind the last one are zero
+// queries -> fragments [blocks][tiles][4][64][8]; the last tile holds the last sixteen queries (moved), or zeros behind the last one
 template<class T>
 __global__ void __launch_bounds__(256) fragment_kernel(const T *query, int64_t query_stride, bool wide, uint32_t num_query, uint32_t tiles, int dim,
-                                                       int blocks, __bf16 *fragments) {
+                                                       int blocks, bool moved, __bf16 *fragments) {
     const uint32_t item = blockIdx.x * 8 + threadIdx.x / 32;  // (row, block)
     const uint32_t row = item / blocks, block = item % blocks;
     if (row >= tiles * 16) return;
     const int c = (threadIdx.x & 31) * 4;
     float x[4] = {0, 0, 0, 0};
-    if (row < num_query) load4(query + (int64_t)row * query_stride, (int)block * kBlockColumns + c, dim, wide, x);
+    const uint32_t from = moved && row / 16 == tiles - 1 ? num_query - 16 + row % 16 : row;
+    if (from < num_query) load4(query + (int64_t)from * query_stride, (int)block * kBlockColumns + c, dim, wide, x);
     put_fragment(fragments + ((size_t)block * tiles + row / 16) * 4 * kFragment, row % 16, c, x);
+}
+
+// what the lanes of a wave wrote to LDS is there for its other lanes (LDS works in order for a wave: this binds the compiler)
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// until this wave's global loads have arrived, those into LDS among them (s_waitcnt vmcnt(0))
+__device__ __forceinline__ void wait_for_loads() {
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    asm volatile("" ::: "memory");
 }
 
 // sixteen bytes of a table row -> the two bf16 operands of steps 2 j and 2 j + 1
@@ -169,19 +183,62 @@ __device__ __forceinline__ void widen(const uint4 raw, float scale, bf16x8 out[2
     }
 }
 
+// 16 queries x 64 candidates of a wave -> logits.  A lane holds 4 x 4 consecutive candidates of one query (acc[i]: candidates
+// 16 i + 4 (lane / 16) ...): stored as they are, an instruction would write 16 rows, 32 or 64 bytes in each.  They turn in the wave's
+// own LDS (rows padded by 16 bytes: no bank conflicts), and an instruction then writes 16 bytes a lane along 4 or 8 rows, 256 or 128
+// bytes in each — measured with the stores alone, 777 x 99991 f16: 29 us against 63, 1024 x 1M f32: 745 against 797.  Rows may begin
+// anywhere: this hardware stores 16 bytes at any address (aligned ones would take 27 us of those 29).
+template<class T>
+struct wave_turn {
+    static constexpr int pitch = 64 * (int)sizeof(T) + 16;
+    uint4 bytes[16 * pitch / 16];
+};
+
+template<bool WHOLE, class T>
+__device__ __forceinline__ void store_turned(wave_turn<T> &turn, T *logits, int64_t logit_stride, uint32_t m0, uint32_t num_query, uint32_t n0, uint32_t num_row,
+                                             const f32x4 acc[4]) {
+    constexpr int E = 16 / (int)sizeof(T), lanes = 64 / E, rows = 64 / lanes;  // lanes to a row's 64 candidates, rows to an instruction
+    const int lane = threadIdx.x & 63;
+    char *const bytes = reinterpret_cast<char *>(turn.bytes);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        T t[4] = {from_float<T>(acc[i][0]), from_float<T>(acc[i][1]), from_float<T>(acc[i][2]), from_float<T>(acc[i][3])};
+        __builtin_memcpy(__builtin_assume_aligned(bytes + (lane & 15) * wave_turn<T>::pitch + (i * 16 + (lane >> 4) * 4) * (int)sizeof(T), 4 * sizeof(T)), t, sizeof(t));
+    }
+    wave_fence();
+#pragma unroll
+    for (int i = 0; i < 16 / rows; i++) {
+        const int row = i * rows + lane / lanes, column = lane % lanes * E;
+        const uint4 raw = *reinterpret_cast<const uint4 *>(bytes + row * wave_turn<T>::pitch + column * (int)sizeof(T));
+        const uint32_t m = m0 + row, n = n0 + column;
+        T *const out = logits + (int64_t)m * logit_stride + n;
+        if constexpr (WHOLE) {
+            __builtin_memcpy(out, &raw, 16);
+            continue;
+        }
+        if (m >= num_query) continue;
+        if (n + E <= num_row) {
+            __builtin_memcpy(out, &raw, 16);
+        } else {
+            T t[E];
+            __builtin_memcpy(t, &raw, 16);
+            for (int r = 0; r < E; r++)
+                if (n + r < num_row) out[r] = t[r];
+        }
+    }
+    wave_fence();  // the next tile turns in the same place
+}
+
 // logits [m][n .. n + 4) of one lane
 template<class T>
-__device__ __forceinline__ void store4(T *row, uint32_t n, uint32_t num_row, bool wide, const f32x4 z) {
-    if (wide && n + 4 <= num_row) {
-        T t[4] = {from_float<T>(z[0]), from_float<T>(z[1]), from_float<T>(z[2]), from_float<T>(z[3])};
-        if constexpr (sizeof(T) == 4)
-            *reinterpret_cast<float4 *>(row + n) = *reinterpret_cast<const float4 *>(t);
-        else
-            *reinterpret_cast<uint2 *>(row + n) = *reinterpret_cast<const uint2 *>(t);
+__device__ __forceinline__ void store4(T *row, uint32_t n, uint32_t num_row, const f32x4 z) {
+    T t[4] = {from_float<T>(z[0]), from_float<T>(z[1]), from_float<T>(z[2]), from_float<T>(z[3])};
+    if (n + 4 <= num_row) {
+        __builtin_memcpy(row + n, t, sizeof(t));
     } else {
 #pragma unroll
         for (int r = 0; r < 4; r++)
-            if (n + r < num_row) row[n + r] = from_float<T>(z[r]);
+            if (n + r < num_row) row[n + r] = t[r];
     }
 }
 
@@ -192,19 +249,29 @@ struct table_view {
     int blocks, padded;  // padded: columns a row holds, dim rounded up to 16
 };
 
-// raw bytes and scales of TILES tiles of 16 table rows, block `block`
-template<int TILES>
-__device__ __forceinline__ void load_table(const table_view &t, uint32_t first, int block, uint4 raw[TILES][2], float scale[TILES]) {
-    const int lane = threadIdx.x & 63, column = block * kBlockColumns + (lane >> 4) * 16;
+// A wave's 64 rows of a table, four tiles of sixteen, as it walks along the columns.  Rows behind the last one are the last one (read, never
+// stored); columns behind a row's end are zero, by a mask after a load that stays inside the row: no branch, so that the
+// compiler counts the loads that are under way.
+struct table_rows {
+    const uint8_t *at[4], *exponent[4];
+    int padded, group;
+
+    __device__ __forceinline__ table_rows(const table_view &t, uint32_t first) : padded(t.padded), group((threadIdx.x & 63) >> 4) {
 #pragma unroll
-    for (int i = 0; i < TILES; i++) {
-        const uint32_t row = min(first + i * 16 + (lane & 15), t.num_row - 1);  // rows behind the last one: read, never stored
-        const uint8_t *at = t.values + (int64_t)row * t.value_stride + column;
-        raw[i][0] = column < t.padded ? *reinterpret_cast<const uint4 *>(at) : uint4{0, 0, 0, 0};
-        raw[i][1] = column + 64 < t.padded ? *reinterpret_cast<const uint4 *>(at + 64) : uint4{0, 0, 0, 0};
-        scale[i] = __uint_as_float((uint32_t)t.exponents[(size_t)row * t.blocks + block] << 23);
+        for (int i = 0; i < 4; i++) {
+            const uint32_t row = min(first + i * 16 + (threadIdx.x & 15), t.num_row - 1);
+            at[i] = t.values + (int64_t)row * t.value_stride;
+            exponent[i] = t.exponents + (size_t)row * t.blocks;
+        }
     }
-}
+    __device__ __forceinline__ uint4 load(int i, int block, int j) const {
+        const int column = block * kBlockColumns + j * 64 + group * 16;
+        const uint4 raw = *reinterpret_cast<const uint4 *>(at[i] + min(column, padded - 16));
+        const uint32_t mask = (uint32_t)((column - padded) >> 31);
+        return uint4{raw.x & mask, raw.y & mask, raw.z & mask, raw.w & mask};
+    }
+    __device__ __forceinline__ float scale(int i, int block) const { return __uint_as_float((uint32_t)exponent[i][block] << 23); }
+};
 
 // up to 16 queries: the table is read once and that bounds it.  Each workgroup lays the queries out for itself (no launch
 // before this one) and walks over strips of 64 candidates per wave.
@@ -212,7 +279,7 @@ constexpr int kFewBlocks = 4;  // 512 columns: 16 KB of fragments
 
 template<class Q, class T>
 __global__ void __launch_bounds__(256) few_queries_kernel(const Q *query, int64_t query_stride, bool query_wide, uint32_t num_query, int dim,
-                                                          table_view table, T *logits, int64_t logit_stride, bool wide) {
+                                                          table_view table, T *logits, int64_t logit_stride) {
     __shared__ __bf16 fragments[kFewBlocks * 4 * kFragment];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int item = threadIdx.x / 32; item < 16 * table.blocks; item += 8) {
@@ -225,10 +292,12 @@ __global__ void __launch_bounds__(256) few_queries_kernel(const Q *query, int64_
     const uint32_t strips = (table.num_row + 63) / 64;
     for (uint32_t strip = blockIdx.x * 4 + wave; strip < strips; strip += gridDim.x * 4) {
         f32x4 acc[4] = {};
+        const table_rows rows(table, strip * 64);
         for (int block = 0; block < table.blocks; block++) {
             uint4 raw[4][2];
             float scale[4];
-            load_table<4>(table, strip * 64, block, raw, scale);
+#pragma unroll
+            for (int i = 0; i < 4; i++) raw[i][0] = rows.load(i, block, 0), raw[i][1] = rows.load(i, block, 1), scale[i] = rows.scale(i, block);
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 bf16x8 b[2];
@@ -246,58 +315,130 @@ __global__ void __launch_bounds__(256) few_queries_kernel(const Q *query, int64_
         const uint32_t m = lane & 15;
         if (m < num_query) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) store4(logits + (int64_t)m * logit_stride, strip * 64 + i * 16 + (lane >> 4) * 4, table.num_row, wide, acc[i]);
+            for (int i = 0; i < 4; i++) store4(logits + (int64_t)m * logit_stride, strip * 64 + i * 16 + (lane >> 4) * 4, table.num_row, acc[i]);
         }
     }
 }
 
-// more queries: a workgroup makes 256 candidates x 16 * TILES queries, 64 candidates to a wave, the queries' fragments of a block
-// of columns in LDS.  The workgroups that share candidates are consecutive on one XCD (its L2 then serves the table's rows).
+// up to 128 columns, 64 candidates and 17 queries or more: what moves is the answer, and the table once.  A wave widens 64 candidates into
+// registers and walks over the queries' tiles, whose fragments (4 KB each, the same for every wave) come through L1: sixteen matrix
+// instructions and 64 x 16 logits a step, no barrier.  Loads and stores of a wave come back in order, so what is loaded behind
+// stores waits until those are in memory: the next tile's fragments are asked for before this tile's logits are stored, and
+// nothing on the way is conditional, so that the wait is for the loads alone (the last tile and the last strip are moved back to
+// end with the rows: some logits are computed twice, to the same bits).
+// Measured at 1024 x 1M x d128: f32 835 us, bf16 478; without the table's loads 773 and 395, the stores alone 745 and 380, in any order
+// of them: the write rate of rows (5.5 TB/s) bounds it, and reads between the writes cost more than their bytes.  Three workgroups
+// to a CU (held by LDS they do not use): with four, the writes of more rows meet, 853 and 492; with two, 911 and 454.  Waves that stay
+// and walk over strips with the queries in LDS: 882 and 476.
+constexpr size_t kThreeToACu = 52 * 1024;
+
+template<class T>
+__global__ void __launch_bounds__(256, 3) narrow_kernel(const __bf16 *fragments, uint32_t tiles, uint32_t num_query, uint32_t parts, table_view table, T *logits,
+                                                        int64_t logit_stride) {
+    __shared__ wave_turn<T> turns[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t xcd = blockIdx.x % 8, turn = blockIdx.x / 8;  // the parts of a strip: consecutive on one XCD
+    const uint32_t part = turn % parts, strip = ((turn / parts) * 8 + xcd) * 4 + wave;
+    if ((uint64_t)strip * 64 >= table.num_row) return;
+    const uint32_t first = min(strip * 64, table.num_row - 64);
+    const table_rows rows(table, first);
+    bf16x8 a[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float scale = rows.scale(i, 0);
+        widen(rows.load(i, 0, 0), scale, a[i]), widen(rows.load(i, 0, 1), scale, a[i] + 2);
+    }
+    const uint32_t begin = (uint32_t)((uint64_t)tiles * part / parts), end = (uint32_t)((uint64_t)tiles * (part + 1) / parts);
+    const bf16x8 *const at = reinterpret_cast<const bf16x8 *>(fragments) + lane;
+    bf16x8 b[4];
+    const auto fetch = [&](uint32_t tile) {
+#pragma unroll
+        for (int s = 0; s < 4; s++) b[s] = at[(size_t)(tile * 4 + s) * 64];
+    };
+    fetch(begin);
+    wait_for_loads();
+    for (uint32_t tile = begin; tile < end; tile++) {
+        f32x4 acc[4] = {};
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i][s], b[s], acc[i], 0, 0, 0);
+        }
+        fetch(min(tile + 1, end - 1));
+        store_turned<true>(turns[wave], logits, logit_stride, min(tile * 16, num_query - 16), num_query, first, table.num_row, acc);
+    }
+}
+
+// more columns: a workgroup makes 256 candidates x 16 * TILES queries, 64 candidates to a wave, the queries' fragments of a block of columns
+// in LDS, those of the next block and its table rows on their way meanwhile.  The workgroups that share candidates are consecutive
+// on one XCD (its L2 then serves the table's rows).
 template<int TILES, class T>
-__global__ void __launch_bounds__(256) logits_kernel(const __bf16 *fragments, uint32_t tiles, uint32_t num_query, table_view table, T *logits,
-                                                     int64_t logit_stride, bool wide) {
-    __shared__ uint4 staged[TILES * 256];
+__global__ void __launch_bounds__(256, 2) logits_kernel(const __bf16 *fragments, uint32_t tiles, uint32_t num_query, table_view table, T *logits,
+                                                        int64_t logit_stride) {
+    // two objects, not one array: the compiler then knows that reading one does not wait for what is on its way into the other
+    constexpr int kTurns = 4 * (int)sizeof(wave_turn<T>) / 16;
+    __shared__ uint4 even[TILES * 256 > kTurns ? TILES * 256 : kTurns], odd[TILES * 256];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t parts = (tiles + TILES - 1) / TILES;
     const uint32_t xcd = blockIdx.x % 8, turn = blockIdx.x / 8;
     const uint32_t part = turn % parts, strip = (turn / parts) * 8 + xcd;
     if ((uint64_t)strip * 256 >= table.num_row) return;  // the whole workgroup
     const uint32_t first = strip * 256 + wave * 64, tile0 = part * TILES;
-    f32x4 acc[4][TILES] = {};
-    for (int block = 0; block < table.blocks; block++) {
-        uint4 raw[4][2];
-        float scale[4];
-        load_table<4>(table, first, block, raw, scale);
-        if (block) __syncthreads();
-        const uint4 *source = reinterpret_cast<const uint4 *>(fragments + ((size_t)block * tiles + tile0) * 4 * kFragment);
-        const uint32_t held = min((uint32_t)TILES, tiles - tile0) * 256;
+    f32x4 acc[TILES][4] = {};
+    const table_rows rows(table, first);
+    uint4 raw[4][2];
+    float scale[4];
+    const auto stage = [&](uint4 *into, int block) {
 #pragma unroll
-        for (int i = 0; i < TILES; i++) staged[i * 256 + threadIdx.x] = i * 256u + threadIdx.x < held ? source[i * 256 + threadIdx.x] : uint4{0, 0, 0, 0};
+        for (int i = 0; i < TILES; i++) {
+            const uint32_t tile = min(tile0 + i, tiles - 1);  // tiles behind the last one: computed, never stored
+            const __bf16 *from = fragments + ((size_t)block * tiles + tile) * 4 * kFragment + threadIdx.x * 8;
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
+                                             (__attribute__((address_space(3))) void *)&into[i * 256 + wave * 64], 16, 0, 0);
+        }
+    };
+    const auto step = [&](const uint4 *staged, uint4 *other, int block) {
+        // this wave's loads into LDS have landed, then everyone's: this block is there, and the one before is done with
+        wait_for_loads();
         __syncthreads();
+        if (block + 1 < table.blocks) stage(other, block + 1);
+        const int after = min(block + 1, table.blocks - 1);
+        float next_scale[4];
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             bf16x8 a[4][2];
 #pragma unroll
             for (int i = 0; i < 4; i++) widen(raw[i][j], scale[i], a[i]);
 #pragma unroll
+            for (int i = 0; i < 4; i++) {
+                raw[i][j] = rows.load(i, after, j);
+                if (j == 0) next_scale[i] = rows.scale(i, after);
+            }
+#pragma unroll
             for (int h = 0; h < 2; h++) {
 #pragma unroll
                 for (int tile = 0; tile < TILES; tile++) {
                     const bf16x8 b = __builtin_bit_cast(bf16x8, staged[(tile * 4 + 2 * j + h) * 64 + lane]);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) acc[i][tile] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i][h], b, acc[i][tile], 0, 0, 0);
+                    for (int i = 0; i < 4; i++) acc[tile][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i][h], b, acc[tile][i], 0, 0, 0);
                 }
             }
         }
-    }
 #pragma unroll
-    for (int tile = 0; tile < TILES; tile++) {
-        const uint32_t m = (tile0 + tile) * 16 + (lane & 15);
-        if (m < num_query) {
+        for (int i = 0; i < 4; i++) scale[i] = next_scale[i];
+    };
+    stage(even, 0);
 #pragma unroll
-            for (int i = 0; i < 4; i++) store4(logits + (int64_t)m * logit_stride, first + i * 16 + (lane >> 4) * 4, table.num_row, wide, acc[i][tile]);
-        }
+    for (int i = 0; i < 4; i++) raw[i][0] = rows.load(i, 0, 0), raw[i][1] = rows.load(i, 0, 1), scale[i] = rows.scale(i, 0);
+    for (int block = 0; block < table.blocks; block += 2) {
+        step(even, odd, block);
+        if (block + 1 < table.blocks) step(odd, even, block + 1);
     }
+    __syncthreads();  // the turns lie over the fragments
+    wave_turn<T> &turned = reinterpret_cast<wave_turn<T> *>(even)[wave];
+#pragma unroll
+    for (int tile = 0; tile < TILES; tile++)
+        store_turned<false>(turned, logits, logit_stride, (tile0 + tile) * 16, num_query, first, table.num_row, acc[tile]);
 }
 
 bool aligned(const void *p, int64_t stride_bytes, size_t to) { return (uintptr_t)p % to == 0 && stride_bytes % (int64_t)to == 0; }
@@ -331,24 +472,33 @@ template<class Q, class T>
 int launch_logits(hipStream_t stream, const Q *query, int64_t query_stride, uint32_t num_query, int dim, const table_view &table, T *logits,
                   int64_t logit_stride, void *workspace) {
     const bool query_wide = aligned(query, query_stride * (int64_t)sizeof(Q), 4 * sizeof(Q));
-    const bool wide = aligned(logits, logit_stride * (int64_t)sizeof(T), 4 * sizeof(T));
-    if (!workspace) {
+    if (num_query <= 16 && table.blocks <= kFewBlocks) {
         const uint32_t groups = (table.num_row + 255) / 256;
         hipLaunchKernelGGL((few_queries_kernel<Q, T>), dim3(groups < 2048 ? groups : 2048), dim3(256), 0, stream, query, query_stride, query_wide,
-                           num_query, dim, table, logits, logit_stride, wide);
+                           num_query, dim, table, logits, logit_stride);
         return launched("gvk_block_logits");
     }
     const uint32_t tiles = (num_query + 15) / 16;
     __bf16 *fragments = reinterpret_cast<__bf16 *>(workspace);
+    const bool narrow = table.blocks == 1 && num_query > 16 && table.num_row >= 64;
     hipLaunchKernelGGL((fragment_kernel<Q>), dim3((tiles * 16 * table.blocks + 7) / 8), dim3(256), 0, stream, query, query_stride, query_wide,
-                       num_query, tiles, dim, table.blocks, fragments);
+                       num_query, tiles, dim, table.blocks, narrow, fragments);
     const uint64_t strips = ((uint64_t)table.num_row + 255) / 256;
+    if (narrow) {
+        // parts of at least eight tiles, until there are eight waves for every SIMD (777 x 99991: 40 us at six parts, 41.6 at four)
+        uint32_t parts = 1;
+        while (strips * parts < 2048 && tiles / (parts * 2) >= 8) parts *= 2;
+        const uint64_t grid = (strips + 7) / 8 * 8 * parts;
+        if (grid > 0xffffffull) return gvk_fail(GVK_EINVAL, "gvk_block_logits: too many logits for one call");
+        hipLaunchKernelGGL((narrow_kernel<T>), dim3((unsigned)grid), dim3(256), kThreeToACu - 4 * sizeof(wave_turn<T>), stream, fragments, tiles, num_query, parts, table, logits, logit_stride);
+        return launched("gvk_block_logits");
+    }
 #define GVK_LOGITS(TILES)                                                                                                                 \
     {                                                                                                                                     \
         const uint64_t grid = (strips + 7) / 8 * 8 * ((tiles + TILES - 1) / TILES);                                                       \
         if (grid > 0xffffffull) return gvk_fail(GVK_EINVAL, "gvk_block_logits: too many logits for one call");                          \
         hipLaunchKernelGGL((logits_kernel<TILES, T>), dim3((unsigned)grid), dim3(256), 0, stream, fragments, tiles, num_query, table, logits, \
-                           logit_stride, wide);                                                                                           \
+                           logit_stride);                                                                                           \
     }
     if (tiles <= 1) GVK_LOGITS(1)
     else if (tiles <= 2) GVK_LOGITS(2)

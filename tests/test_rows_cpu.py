@@ -61,9 +61,10 @@ def test_block_entry_points_refuse(lib):
     refused(lib, logits(query=None), "null")
     refused(lib, logits(z=None), "null")
     refused(lib, logits(values=None), "null")
-    refused(lib, logits(m=17), "workspace")
-    refused(lib, logits(m=17, space=P, nbytes=8191), "workspace of 8192")
-    refused(lib, logits(m=17, space=C.c_void_p((1 << 20) + 4), nbytes=8192), "workspace")
+    many = dict(m=17, dim=200, qstride=200, vstride=208)
+    refused(lib, logits(**many), "workspace")
+    refused(lib, logits(space=P, nbytes=16383, **many), "workspace of 16384")
+    refused(lib, logits(space=C.c_void_p((1 << 20) + 4), nbytes=16384, **many), "workspace")
     assert logits(m=0) == 0 and logits(n=0, zstride=0) == 0
     assert lib.gvk_block_logits_workspace(16, 512) == 0 and lib.gvk_block_logits_workspace(16, 513) == 5 * 4096
     assert lib.gvk_block_logits_workspace(1000, 96) == 63 * 4096
