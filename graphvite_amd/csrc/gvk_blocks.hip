@@ -24,6 +24,7 @@ namespace {
 
 using gvk_rows::from_float;
 using gvk_rows::to_float;
+using gvk_rows::wave_fence;
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -154,13 +155,6 @@ __global__ void __launch_bounds__(256) fragment_kernel(const T *query, int64_t q
     const uint32_t from = moved && row / 16 == tiles - 1 ? num_query - 16 + row % 16 : row;
     if (from < num_query) load4(query + (int64_t)from * query_stride, (int)block * kBlockColumns + c, dim, wide, x);
     put_fragment(fragments + ((size_t)block * tiles + row / 16) * 4 * kFragment, row % 16, c, x);
-}
-
-// what the lanes of a wave wrote to LDS is there for its other lanes (LDS works in order for a wave: this binds the compiler)
-__device__ __forceinline__ void wave_fence() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 // until this wave's global loads have arrived, those into LDS among them (s_waitcnt vmcnt(0))

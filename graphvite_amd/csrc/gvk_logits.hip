@@ -28,13 +28,16 @@ __device__ __forceinline__ float reference_of(float largest) { return largest ==
 
 // ---- the top of a row ---------------------------------------------------------------------------------------------------------
 // Entries are ordered by (logit, lower candidate first): one 64-bit key, unique in a row, so whatever order candidates are
-// collected in, the answer is the same.  A slice of a row lives in the registers of a workgroup.  The largest of every thread's
-// elements gives a bound: of each wave's 64 such maxima the ceil(k / waves)-th largest, and of those the least.  At least k
-// elements reach it, and only a few more than k do (16384 normal logits, k = 64: about 90), so they fit in LDS and are ranked by
-// counting.  Rows that defeat the bound (all logits equal, NaN) take the exact way: a bisection of the key, bit by bit.
+// collected in, the answer is the same.  A slice of a row (16384 logits) lives in the registers of a workgroup.  Every thread takes
+// the largest of its elements (of each quarter of them for k above 128); of a wave's 64 (256) such maxima the ceil(k / waves)-th
+// largest, and of those the least, is a bound that at least k elements reach, and only a few more than k do (normal logits,
+// k = 64: about 85).  Every lane puts those of its own into its own slots in LDS; then they are packed.  One slice: they are ranked by
+// counting.  More: they go to a list, and one workgroup per row does the same with the lists.  Rows that defeat the bound (all logits equal,
+// NaN) take the exact way: a bisection of the key, bit by bit.
 
-constexpr int kTopThreads = 256, kTopWaves = kTopThreads / 64, kTopBuffer = 2048;
-constexpr int kMergeThreads = 512;
+constexpr int kTopThreads = 256, kTopWaves = kTopThreads / 64, kMergeThreads = 512, kMergeWaves = kMergeThreads / 64;
+constexpr uint32_t kPacked = 1024;  // keys a workgroup packs
+constexpr int kSlots = 8;           // slots of a lane
 
 __device__ __forceinline__ uint32_t ordered(float x) {
     if (x != x) return 0xffffffffu;  // NaN above everything: it shows
@@ -46,52 +49,59 @@ __device__ __forceinline__ float of_ordered(uint32_t key) { return __uint_as_flo
 
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t index) { return (uint64_t)ordered(x) << 32 | (uint32_t)~index; }
 
-// the rank-th largest (1-based) of the 64 values a wave holds, its lowest 16 bits cut off: a bound that `rank` of them reach
-__device__ __forceinline__ uint32_t wave_bound(uint32_t value, int rank) {
+// the rank-th largest (1-based) of the 64 * N values a wave holds, its lowest 16 bits cut off: a bound that `rank` of them reach (0: not
+// that many do)
+template<int N>
+__device__ __forceinline__ uint32_t wave_bound(const uint32_t (&value)[N], int rank) {
     uint32_t bound = 0;
 #pragma unroll
     for (int bit = 31; bit >= 16; bit--) {
         const uint32_t trial = bound | 1u << bit;
-        if (__popcll(__ballot(value >= trial)) >= rank) bound = trial;
+        int count = 0;
+#pragma unroll
+        for (int i = 0; i < N; i++) count += __popcll(__ballot(value[i] >= trial));
+        if (count >= rank) bound = trial;
     }
     return bound;
 }
 
+template<int WAVES>
 struct top_shared {
-    uint64_t keys[kTopBuffer];
-    uint32_t bound[kMergeThreads / 64];
-    float reduce[kMergeThreads / 64];
-    uint32_t count, exact;
+    uint64_t packed[kPacked + 8];
+    uint32_t count;  // of packed keys, beyond what fits, so that it is known
+    uint32_t bound[WAVES];
+    float reduce[WAVES], sum[WAVES];
 };
 
-// keys[0 .. count) -> the k largest in order, by counting the larger ones
-template<int THREADS, class Write>
-__device__ __forceinline__ void write_ranked(const top_shared &s, uint32_t count, uint32_t k, Write write) {
-    for (uint32_t i = threadIdx.x; i < count; i += THREADS) {
-        const uint64_t key = s.keys[i];
+// Lanes with a key of a wave append it.
+template<int WAVES>
+__device__ __forceinline__ void append(top_shared<WAVES> &s, bool mine, uint64_t key) {
+    const uint64_t all = __ballot(mine);
+    uint32_t base = 0;
+    if ((threadIdx.x & 63) == 0) base = atomicAdd(&s.count, (uint32_t)__popcll(all));
+    base = __builtin_amdgcn_readfirstlane(base);
+    const uint32_t place = base + __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0));
+    if (mine && place < kPacked) s.packed[place] = key;
+}
+
+// the packed keys -> the k largest in order, by counting the larger ones
+template<int WAVES, class Write>
+__device__ __forceinline__ void write_ranked(top_shared<WAVES> &s, uint32_t count, uint32_t k, Write write) {
+    if (threadIdx.x < 8) s.packed[count + threadIdx.x] = 0;  // whole eights
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < count; i += WAVES * 64) {
+        const uint64_t key = s.packed[i];
         uint32_t rank = 0;
-        for (uint32_t j = 0; j < count; j++) rank += s.keys[j] > key;
+        for (uint32_t j = 0; j < count; j += 8) {
+#pragma unroll
+            for (int u = 0; u < 8; u++) rank += s.packed[j + u] > key;
+        }
         if (rank < k) write(rank, key);
     }
 }
 
-// The least threshold found, from the highest bit down, that at least `want` keys reach and that leaves no more than fit the
-// buffer; count_reaching(threshold) counts over the workgroup.  All 64 bits end at the want-th largest key itself.
-template<class Count>
-__device__ __forceinline__ uint64_t exact_threshold(uint32_t want, Count count_reaching) {
-    uint64_t threshold = 0;
-    for (int bit = 63; bit >= 0; bit--) {
-        const uint64_t trial = threshold | 1ull << bit;
-        const uint32_t count = count_reaching(trial);
-        if (count < want) continue;
-        threshold = trial;
-        if (count <= (uint32_t)kTopBuffer) break;
-    }
-    return threshold;
-}
-
-template<int THREADS>
-__device__ __forceinline__ uint32_t block_count(uint32_t v, top_shared &s) {
+template<int WAVES>
+__device__ __forceinline__ uint32_t block_count(uint32_t v, top_shared<WAVES> &s) {
 #pragma unroll
     for (int step = 1; step < 64; step <<= 1) v += __shfl_xor((int)v, step);
     __syncthreads();
@@ -99,8 +109,75 @@ __device__ __forceinline__ uint32_t block_count(uint32_t v, top_shared &s) {
     __syncthreads();
     v = 0;
 #pragma unroll
-    for (int i = 0; i < THREADS / 64; i++) v += s.bound[i];
+    for (int i = 0; i < WAVES; i++) v += s.bound[i];
     return v;
+}
+
+// The exact way.  The least threshold found, from the highest bit down, that at least `want` keys reach and no more than can be packed; all
+// 64 bits end at the want-th largest key itself.  Then those keys, packed.
+template<int WAVES, class Each>
+__device__ __forceinline__ uint32_t collect_exactly(top_shared<WAVES> &s, uint32_t want, Each each) {
+    uint64_t threshold = 0;
+    for (int bit = 63; bit >= 0; bit--) {
+        const uint64_t trial = threshold | 1ull << bit;
+        uint32_t reached = 0;
+        each([&](bool valid, uint64_t key) { reached += valid && key >= trial; });
+        reached = block_count(reached, s);
+        if (reached < want) continue;
+        threshold = trial;
+        if (reached <= kPacked) break;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) s.count = 0;
+    __syncthreads();
+    each([&](bool valid, uint64_t key) { append(s, valid && key >= threshold, key); });
+    __syncthreads();
+    return min(s.count, kPacked);
+}
+
+// For each of N parts of a thread's elements one of them, as large as comes cheap: the largest, or — bf16, compared two at a time as 16-bit
+// whole numbers — the largest where any is positive, else some element.
+template<class T>
+constexpr bool representative_is_largest() { return !__is_same(T, __bf16); }
+
+template<class T, int U, int N>
+__device__ __forceinline__ void representatives(const uint4 (&raw)[U], float (&part)[N]) {
+    constexpr int E = per_chunk<T>::value;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < N; i++) part[i] = -kInfinity;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            float x[E];
+            unpack<T>(raw[u], x);
+#pragma unroll
+            for (int i = 0; i < E; i++) part[(u * E + i) * N / (U * E)] = fmaxf(part[(u * E + i) * N / (U * E)], x[i]);
+        }
+    } else {
+        typedef short pair_bits __attribute__((ext_vector_type(2)));
+        typedef _Float16 pair_f16 __attribute__((ext_vector_type(2)));
+        uint32_t best[N];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const uint32_t word[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                constexpr int words = U * 4 / N;
+                const int p = (u * 4 + i) / words;
+                if ((u * 4 + i) % words == 0) best[p] = word[i];
+                else if constexpr (__is_same(T, __bf16))
+                    best[p] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(pair_bits, best[p]), __builtin_bit_cast(pair_bits, word[i])));
+                else
+                    best[p] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(pair_f16, best[p]), __builtin_bit_cast(pair_f16, word[i])));
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < N; p++) {
+            T t[2];
+            __builtin_memcpy(t, &best[p], 4);
+            part[p] = fmaxf(to_float(t[0]), to_float(t[1]));
+        }
+    }
 }
 
 struct top_output {
@@ -112,93 +189,102 @@ struct top_output {
     float2 *partial;   // [rows][slices]
 };
 
-// One slice of one row: U chunks to a thread, in registers.
-template<class T, int U>
+// One slice of one row: U chunks to a thread, in registers; N maxima to a thread.
+template<class T, int U, int N>
 __global__ void __launch_bounds__(kTopThreads) top_kernel(const T *logits, int64_t stride, int64_t first_row, uint32_t slices, int64_t num_col, uint32_t k,
                                                           uint32_t capacity, float scale, top_output out) {
     constexpr int E = per_chunk<T>::value;
-    __shared__ top_shared s;
+    __shared__ top_shared<kTopWaves> s;
+    __shared__ uint64_t slots[kSlots][kTopThreads];
     const int64_t row = first_row + blockIdx.x / slices;
-    const uint32_t slice = blockIdx.x % slices;
+    const uint32_t slice = blockIdx.x % slices, wave = threadIdx.x >> 6;
     const chunked_row<T> z(logits + row * stride, num_col);
-    const int64_t chunk0 = (int64_t)slice * U * kTopThreads;
+    // slices of equal length, in whole cache lines: a short last one would give few maxima and a poor bound
+    const int64_t chunks = z.chunks(), share = ((chunks + slices - 1) / slices + 7) & ~(int64_t)7;
+    const int64_t chunk0 = min(chunks, share * slice), chunk1 = min(chunks, chunk0 + share);
+    const auto load = [&](int u) {
+        const int64_t chunk = chunk0 + u * kTopThreads + threadIdx.x;
+        return z.load(chunk < chunk1 ? chunk : chunks);  // the one behind the last reads as minus infinity
+    };
     uint4 raw[U];
 #pragma unroll
-    for (int u = 0; u < U; u++) raw[u] = z.load(chunk0 + u * kTopThreads + threadIdx.x);
-    if (threadIdx.x == 0) s.count = 0, s.exact = 0;
+    for (int u = 0; u < U; u++) raw[u] = load(u);
 
-    float largest = -kInfinity;
+    float part[N];
+    representatives<T>(raw, part);
+    float largest = part[0];
+    uint32_t part_ordered[N];
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        float x[E];
-        unpack<T>(raw[u], x);
-#pragma unroll
-        for (int i = 0; i < E; i++) largest = fmaxf(largest, x[i]);
-    }
-    const uint32_t wave_share = (k + kTopWaves - 1) / kTopWaves;
-    const uint32_t bound = wave_bound(ordered(largest), (int)wave_share);
-    if ((threadIdx.x & 63) == 0) s.bound[threadIdx.x >> 6] = bound;
-    const float m = block_max<kTopThreads>(largest, s.reduce);  // its barriers publish the bounds too
+    for (int i = 0; i < N; i++) part_ordered[i] = ordered(part[i]), largest = fmaxf(largest, part[i]);
+    const uint32_t bound = wave_bound(part_ordered, (int)((k + kTopWaves - 1) / kTopWaves));
+    largest = wave_max(largest);
+    if ((threadIdx.x & 63) == 0) s.bound[wave] = bound, s.reduce[wave] = largest;
+    if (threadIdx.x == 0) s.count = 0;
+    __syncthreads();
+    float m = s.reduce[0];
     uint32_t least = s.bound[0];
 #pragma unroll
-    for (int w = 1; w < kTopWaves; w++) least = min(least, s.bound[w]);
+    for (int w = 1; w < kTopWaves; w++) least = min(least, s.bound[w]), m = fmaxf(m, s.reduce[w]);
+    if (!representative_is_largest<T>() && m < 0) {  // the whole slice below zero: once more, as numbers
+        largest = -kInfinity;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            float x[E];
+            unpack<T>(raw[u], x);
+#pragma unroll
+            for (int i = 0; i < E; i++) largest = fmaxf(largest, x[i]);
+        }
+        m = block_max<kTopThreads>(largest, s.reduce);
+    }
     // cut bits may make a NaN of minus infinity's key
     const float tau = least <= 0x007fffffu ? -kInfinity : of_ordered(least);
     const float base = reference_of(m);
     float sum = 0;
+    // What reaches the bound is put down as it is, with its place in the slice (what lies outside the row is minus infinity and does not
+    // reach a bound above that); the keys are made of it afterwards.
+    uint32_t mine = 0;
 #pragma unroll
     for (int u = 0; u < U; u++) {
         float x[E];
         unpack<T>(raw[u], x);
-        const int64_t at = z.first(chunk0 + u * kTopThreads + threadIdx.x);
 #pragma unroll
         for (int i = 0; i < E; i++) {
             sum += exp2_fast((x[i] - base) * scale);
-            if (x[i] >= tau && at + i >= 0 && at + i < num_col) {
-                const uint32_t place = atomicAdd(&s.count, 1u);
-                if (place < (uint32_t)kTopBuffer) s.keys[place] = key_of(x[i], (uint32_t)(at + i));
+            if (x[i] >= tau) {
+                slots[min(mine, (uint32_t)kSlots - 1)][threadIdx.x] = (uint64_t)__float_as_uint(x[i]) << 32 | (uint32_t)((u * kTopThreads + threadIdx.x) * E + i);
+                mine++;
             }
         }
     }
-    sum = block_sum<kTopThreads>(sum, s.reduce);
-    uint32_t count = s.count;  // behind the barriers of the sum
-    if (count > (uint32_t)kTopBuffer || sum != sum) {
-        const int64_t begin = max((int64_t)0, z.first(chunk0)), end = min(num_col, z.first(chunk0 + (int64_t)U * kTopThreads));
-        const uint32_t want = (uint32_t)min((int64_t)k, max((int64_t)0, end - begin));
-        auto each = [&](auto visit) {
-#pragma unroll 1
-            for (int u = 0; u < U; u++) {
-                uint4 r = raw[0];
+    const uint32_t origin = (uint32_t)z.first(chunk0);
+    for (uint32_t slot = 0; __any(slot < mine) && slot < kSlots; slot++) {
+        const uint64_t it = slots[slot][threadIdx.x];
+        append(s, slot < mine, key_of(__uint_as_float((uint32_t)(it >> 32)), origin + (uint32_t)it));
+    }
+    const bool full = __any(mine > kSlots);
+    sum = wave_sum(sum);
+    if ((threadIdx.x & 63) == 0) s.sum[wave] = full ? __builtin_nanf("") : sum, s.reduce[wave] = sum;
+    __syncthreads();
+    float check = s.sum[0];
+    sum = s.reduce[0];
 #pragma unroll
-                for (int v = 1; v < U; v++)
-                    if (v == u) r = raw[v];
+    for (int w = 1; w < kTopWaves; w++) sum += s.reduce[w], check += s.sum[w];
+    uint32_t count = s.count;
+    if (count > kPacked || check != check || tau == -kInfinity) {
+        const int64_t begin = max((int64_t)0, z.first(chunk0)), end = min(num_col, z.first(chunk1));
+        count = collect_exactly(s, (uint32_t)min((int64_t)k, max((int64_t)0, end - begin)), [&](auto visit) {
+#pragma unroll 1
+            for (int u = 0; u < U; u++) {  // read again: registers take no index
                 float x[E];
-                unpack<T>(r, x);
+                unpack<T>(load(u), x);
                 const int64_t at = z.first(chunk0 + u * kTopThreads + threadIdx.x);
 #pragma unroll
-                for (int i = 0; i < E; i++)
-                    if (at + i >= 0 && at + i < num_col) visit(key_of(x[i], (uint32_t)(at + i)));
-            }
-        };
-        const uint64_t threshold = exact_threshold(want, [&](uint64_t trial) {
-            uint32_t mine = 0;
-            each([&](uint64_t key) { mine += key >= trial; });
-            return block_count<kTopThreads>(mine, s);
-        });
-        __syncthreads();
-        if (threadIdx.x == 0) s.count = 0;
-        __syncthreads();
-        each([&](uint64_t key) {
-            if (key >= threshold) {
-                const uint32_t place = atomicAdd(&s.count, 1u);
-                if (place < (uint32_t)kTopBuffer) s.keys[place] = key;
+                for (int i = 0; i < E; i++) visit(at + i >= 0 && at + i < end, key_of(x[i], (uint32_t)(at + i)));
             }
         });
-        __syncthreads();
-        count = min(s.count, (uint32_t)kTopBuffer);
     }
     if (slices == 1) {
-        write_ranked<kTopThreads>(s, count, k, [&](uint32_t rank, uint64_t key) {
+        write_ranked(s, count, k, [&](uint32_t rank, uint64_t key) {
             out.values[row * k + rank] = of_ordered((uint32_t)(key >> 32));
             out.index[row * k + rank] = (int32_t)~(uint32_t)key;
         });
@@ -206,73 +292,70 @@ __global__ void __launch_bounds__(kTopThreads) top_kernel(const T *logits, int64
         return;
     }
     const uint64_t list = (uint64_t)blockIdx.x;
-    uint64_t *keys = out.lists + list * capacity;
+    uint64_t *const keys = out.lists + list * capacity;
     if (count <= capacity) {
-        for (uint32_t i = threadIdx.x; i < count; i += kTopThreads) keys[i] = s.keys[i];
+        for (uint32_t i = threadIdx.x; i < count; i += kTopThreads) keys[i] = s.packed[i];
     } else {
-        write_ranked<kTopThreads>(s, count, k, [&](uint32_t rank, uint64_t key) { keys[rank] = key; });
+        write_ranked(s, count, k, [&](uint32_t rank, uint64_t key) { keys[rank] = key; });
         count = k;
     }
     if (threadIdx.x == 0) out.counts[list] = count, out.partial[list] = make_float2(m, sum);
 }
 
-// The lists of a row's slices -> its top entries and statistics.
+// The lists of a row's slices -> its top entries and statistics.  A wave takes every eighth list, several at a time; the bound is the k-th
+// largest of all threads' largest keys (waves have lists of different lengths, or none).
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(int64_t first_row, uint32_t slices, uint32_t k, uint32_t log_capacity, float scale, top_output out) {
-    __shared__ top_shared s;
+    __shared__ top_shared<kMergeWaves> s;
+    __shared__ uint32_t maxima[kMergeThreads];
     const int64_t row = first_row + blockIdx.x;
     const uint64_t list0 = (uint64_t)blockIdx.x * slices;
-    const uint64_t *keys = out.lists + (list0 << log_capacity);
-    const uint32_t *counts = out.counts + list0;
-    const uint64_t total = (uint64_t)slices << log_capacity;
-    const uint32_t mask = (1u << log_capacity) - 1;
-    auto each = [&](auto visit) {
-        for (uint64_t i = threadIdx.x; i < total; i += kMergeThreads)
-            if ((uint32_t)(i & mask) < counts[i >> log_capacity]) visit(keys[i]);
+    const uint64_t *const keys = out.lists + (list0 << log_capacity);
+    const uint32_t *const counts = out.counts + list0;
+    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const auto each = [&](auto visit) {
+        constexpr int kTogether = 4;
+        for (uint32_t l = wave; l < slices; l += kMergeWaves * kTogether) {
+            uint32_t count[kTogether], longest = 0;
+#pragma unroll
+            for (int t = 0; t < kTogether; t++) {
+                count[t] = l + t * kMergeWaves < slices ? counts[l + t * kMergeWaves] : 0;
+                longest = max(longest, count[t]);
+            }
+            for (uint32_t j = lane; j < ((longest + 63) & ~63u); j += 64) {
+                uint64_t key[kTogether];
+#pragma unroll
+                for (int t = 0; t < kTogether; t++) key[t] = j < count[t] ? keys[((uint64_t)(l + t * kMergeWaves) << log_capacity) + j] : 0;
+#pragma unroll
+                for (int t = 0; t < kTogether; t++) visit(j < count[t], key[t]);
+            }
+        }
     };
     if (threadIdx.x == 0) s.count = 0;
     uint32_t largest = 0;
-    each([&](uint64_t key) { largest = max(largest, (uint32_t)(key >> 32)); });
-    const uint32_t bound = wave_bound(largest, (int)((k + kMergeThreads / 64 - 1) / (kMergeThreads / 64)));
-    if ((threadIdx.x & 63) == 0) s.bound[threadIdx.x >> 6] = bound;
+    each([&](bool valid, uint64_t key) {
+        if (valid) largest = max(largest, (uint32_t)(key >> 32));
+    });
+    maxima[threadIdx.x] = largest;
     float m = -kInfinity, sum = 0;
     for (uint32_t i = threadIdx.x; i < slices; i += kMergeThreads) m = fmaxf(m, out.partial[list0 + i].x);
-    m = block_max<kMergeThreads>(m, s.reduce);
+    m = block_max<kMergeThreads>(m, s.reduce);  // its barriers publish the maxima too
     const float base = reference_of(m);
     for (uint32_t i = threadIdx.x; i < slices; i += kMergeThreads) {
         const float2 p = out.partial[list0 + i];
         if (p.x > -kInfinity || p.y != p.y) sum += p.y * exp2_fast((reference_of(p.x) - base) * scale);  // not a slice of nothing but masks
     }
-    sum = block_sum<kMergeThreads>(sum, s.reduce);
-    uint32_t least = s.bound[0];
+    uint32_t all[kMergeWaves];
 #pragma unroll
-    for (int w = 1; w < kMergeThreads / 64; w++) least = min(least, s.bound[w]);
-    each([&](uint64_t key) {
-        if ((uint32_t)(key >> 32) >= least) {
-            const uint32_t place = atomicAdd(&s.count, 1u);
-            if (place < (uint32_t)kTopBuffer) s.keys[place] = key;
-        }
+    for (int i = 0; i < kMergeWaves; i++) all[i] = maxima[i * 64 + lane];
+    const uint32_t least = wave_bound(all, (int)k);
+    each([&](bool valid, uint64_t key) {
+        const bool reaches = valid && (uint32_t)(key >> 32) >= least;
+        if (__any(reaches)) append(s, reaches, key);
     });
-    __syncthreads();
+    sum = block_sum<kMergeThreads>(sum, s.reduce);  // its barriers publish the keys and their count
     uint32_t count = s.count;
-    if (count > (uint32_t)kTopBuffer) {
-        const uint64_t threshold = exact_threshold(k, [&](uint64_t trial) {
-            uint32_t mine = 0;
-            each([&](uint64_t key) { mine += key >= trial; });
-            return block_count<kMergeThreads>(mine, s);
-        });
-        __syncthreads();
-        if (threadIdx.x == 0) s.count = 0;
-        __syncthreads();
-        each([&](uint64_t key) {
-            if (key >= threshold) {
-                const uint32_t place = atomicAdd(&s.count, 1u);
-                if (place < (uint32_t)kTopBuffer) s.keys[place] = key;
-            }
-        });
-        __syncthreads();
-        count = min(s.count, (uint32_t)kTopBuffer);
-    }
-    write_ranked<kMergeThreads>(s, count, k, [&](uint32_t rank, uint64_t key) {
+    if (count > kPacked) count = collect_exactly(s, k, each);
+    write_ranked(s, count, k, [&](uint32_t rank, uint64_t key) {
         out.values[row * k + rank] = of_ordered((uint32_t)(key >> 32));
         out.index[row * k + rank] = (int32_t)~(uint32_t)key;
     });
@@ -644,12 +727,7 @@ top_plan plan_top(int dtype, int64_t num_row, int64_t num_col, int k) {
     top_plan p;
     p.slice = kTopSlice;
     p.slices = slices_of(num_col, p.slice, per_chunk);
-    if (p.slices > 1 && num_row * p.slices < 512) {  // few rows: more, smaller slices, to reach every CU
-        p.slice = kTopSmallSlice;
-        p.slices = slices_of(num_col, p.slice, per_chunk);
-    } else if (slices_of(num_col, kTopSmallSlice, per_chunk) == 1) {
-        p.slice = kTopSmallSlice, p.slices = 1;
-    }
+    if (slices_of(num_col, kTopSmallSlice, per_chunk) == 1) p.slice = kTopSmallSlice, p.slices = 1;
     p.log_capacity = 6;
     while ((1 << p.log_capacity) < 2 * k) p.log_capacity++;
     p.bytes = p.slices > 1 ? (size_t)num_row * p.slices * ((8ull << p.log_capacity) + sizeof(float2) + sizeof(uint32_t)) : 0;
@@ -661,10 +739,14 @@ void launch_top(hipStream_t stream, const top_plan &p, const T *logits, int64_t 
                 const top_output &out) {
     constexpr int E = per_chunk<T>::value, kLarge = kTopSlice / kTopThreads / E, kSmall = kTopSmallSlice / kTopThreads / E;
     const dim3 grid((unsigned)(num_row * p.slices));
-    if (p.slice == kTopSlice)
-        hipLaunchKernelGGL((top_kernel<T, kLarge>), grid, dim3(kTopThreads), 0, stream, logits, stride, first_row, (uint32_t)p.slices, num_col, (uint32_t)k, 1u << p.log_capacity, scale, out);
-    else
-        hipLaunchKernelGGL((top_kernel<T, kSmall>), grid, dim3(kTopThreads), 0, stream, logits, stride, first_row, (uint32_t)p.slices, num_col, (uint32_t)k, 1u << p.log_capacity, scale, out);
+#define GVK_TOP(U, N)                                                                                                                              \
+    hipLaunchKernelGGL((top_kernel<T, U, N>), grid, dim3(kTopThreads), 0, stream, logits, stride, first_row, (uint32_t)p.slices, num_col, (uint32_t)k, \
+                       1u << p.log_capacity, scale, out)
+    if (p.slice == kTopSlice && k <= 128) GVK_TOP(kLarge, 1);
+    else if (p.slice == kTopSlice) GVK_TOP(kLarge, 4);
+    else if (k <= 128) GVK_TOP(kSmall, 1);
+    else GVK_TOP(kSmall, 4);
+#undef GVK_TOP
     if (p.slices > 1)
         hipLaunchKernelGGL(merge_kernel, dim3((unsigned)num_row), dim3(kMergeThreads), 0, stream, first_row, (uint32_t)p.slices, (uint32_t)k, (uint32_t)p.log_capacity, scale, out);
 }

@@ -71,11 +71,41 @@ __device__ __forceinline__ void store_chunk(T *row, int64_t at, int64_t n, bool 
     }
 }
 
+// what the lanes of a wave wrote to LDS is there for its other lanes (LDS works in order for a wave: this binds the compiler)
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// max / sum over a wave, every lane gets it: four steps inside rows of 16 lanes by DPP, two across them
+template<int CONTROL>
+__device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CONTROL, 0xf, 0xf, true));
+}
+
+template<class Op>
+__device__ __forceinline__ float wave_reduce(float v, Op op) {
+    v = op(v, dpp<0xb1>(v));   // quad_perm [1 0 3 2]
+    v = op(v, dpp<0x4e>(v));   // quad_perm [2 3 0 1]
+    v = op(v, dpp<0x141>(v));  // row_half_mirror
+    v = op(v, dpp<0x140>(v));  // row_mirror
+    v = op(v, __shfl_xor(v, 16));
+    return op(v, __shfl_xor(v, 32));
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+    return wave_reduce(v, [](float a, float b) { return fmaxf(a, b); });
+}
+
+__device__ __forceinline__ float wave_sum(float v) {
+    return wave_reduce(v, [](float a, float b) { return a + b; });
+}
+
 // max / sum over a workgroup of THREADS threads, every thread gets it; `shared` holds THREADS / 64 floats.  Fixed order.
 template<int THREADS>
 __device__ __forceinline__ float block_max(float v, float *shared) {
-#pragma unroll
-    for (int step = 1; step < 64; step <<= 1) v = fmaxf(v, __shfl_xor(v, step));
+    v = wave_max(v);
     __syncthreads();  // the last use of `shared` is over
     if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
     __syncthreads();
@@ -87,8 +117,7 @@ __device__ __forceinline__ float block_max(float v, float *shared) {
 
 template<int THREADS>
 __device__ __forceinline__ float block_sum(float v, float *shared) {
-#pragma unroll
-    for (int step = 1; step < 64; step <<= 1) v += __shfl_xor(v, step);
+    v = wave_sum(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
     __syncthreads();
