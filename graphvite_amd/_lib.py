@@ -175,8 +175,10 @@ def lib():
     l.gvk_distill_workspace.argtypes = [i32, wide, wide, i32]
     l.gvk_distill.restype = i32
     l.gvk_distill.argtypes = [vp, i32, vp, wide, wide, wide, i32, vp, vp, vp, f32, vp, vp, vp, vp, wide, vp, C.c_size_t]
+    l.gvk_distill_grad_workspace.restype = C.c_size_t
+    l.gvk_distill_grad_workspace.argtypes = [i32, wide, wide, i32]
     l.gvk_distill_grad.restype = i32
-    l.gvk_distill_grad.argtypes = [vp, i32, vp, wide, wide, wide, i32, vp, vp, vp, f32, vp, vp, vp, wide]
+    l.gvk_distill_grad.argtypes = [vp, i32, vp, wide, wide, wide, i32, vp, vp, vp, f32, vp, vp, vp, wide, vp, C.c_size_t]
     l.gvk_probe_row_traffic.restype = i32
     l.gvk_probe_row_traffic.argtypes = [vp, i32, vp, vp, vp, vp, C.c_float, i32]
     l.gvk_alias_sample.restype = i32

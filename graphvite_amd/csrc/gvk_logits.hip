@@ -246,6 +246,8 @@ __global__ void __launch_bounds__(kTopThreads) top_kernel(const T *logits, int64
 #pragma unroll
     for (int u = 0; u < U; u++) {
         float x[E];
+        // 16-bit logits are unpacked again, rather than kept unpacked: 78 registers, not 152 (1024 x 1M bf16: 577 us against 631)
+        if constexpr (sizeof(T) == 2) asm volatile("" : "+v"(raw[u].x), "+v"(raw[u].y), "+v"(raw[u].z), "+v"(raw[u].w), "+v"(sum));
         unpack<T>(raw[u], x);
 #pragma unroll
         for (int i = 0; i < E; i++) {
@@ -381,114 +383,135 @@ struct distill_output {
     float *loss, *stats;
     void *grad;
     int64_t grad_stride;
-    float2 *partial;  // [rows][slices]
-    float *listed;    // [rows][k]: the student's logits of the list (the gradient may lie over the logits)
+    // workspace of rows longer than a workgroup holds
+    float2 *partial;   // [rows][slices]: max and sum
+    float4 *factors;   // [rows]: what the exponent subtracts, w Q / (T S), 0 or NaN to add, and whether there is nothing to learn
+    int32_t *index;    // [rows][k]: candidates with a share of q, each once; -1: none
+    float *q;          // [rows][k]: w q / T
 };
 
+template<int THREADS>
 struct list_shared {
     int32_t index[kMaxList];  // -1 where the list has no entry
-    float q[kMaxList];
-    float reduce[16];
-    uint32_t bad, any;
+    float q[kMaxList];        // first the logits, then the probabilities
+    float largest[THREADS / 64], listed[THREADS / 64], sum[THREADS / 64], listed_sum[THREADS / 64], q_total[THREADS / 64], loss[THREADS / 64];
+    uint32_t bad[THREADS / 64], any[THREADS / 64], repeated[THREADS / 64];
 };
 
-// The list of a row into LDS: q_e of its entries; returns Q, and log St and mt through the pointers.  An index outside the row makes
-// the row's answer NaN: it shows, and nothing is read or written out of bounds.
-template<int THREADS>
-__device__ __forceinline__ float load_list(const distill_input &in, int64_t row, list_shared &s, float *log_total, float *reference) {
-    if (threadIdx.x == 0) s.bad = 0, s.any = 0;
-    __syncthreads();
-    const int32_t *index = in.index + row * in.k;
-    const float *teacher = in.teacher + row * in.k;
-    float largest = -kInfinity;
+struct row_answer {
+    float m, sum, log_sum, q_total, loss;
+    bool nothing, repeated;
+};
+
+// A row and its list, by a workgroup: three reductions of two numbers each, three barriers.
+//   largest() / sum(base)   a thread's part of max z and of S
+//   seen(i)                 whether candidate i was listed before (by an entry that got there first)
+//   logit(i)                z_i
+//   place(i, q)             called for every entry with its probability, before the last barrier
+// An index outside the row makes the row's answer NaN: it shows, and nothing is read or written out of bounds.  Nothing is to be
+// learned from a row without entries, whatever its logits hold, nor from one whose candidates are all masked: loss and gradient 0.
+template<int THREADS, class Largest, class Sum, class Seen, class Logit, class Place>
+__device__ __forceinline__ row_answer solve_row(const distill_input &in, int64_t row, list_shared<THREADS> &s, Largest largest, Sum sum, Seen seen, Logit logit, Place place) {
+    constexpr int WAVES = THREADS / 64;
+    const uint32_t wave = threadIdx.x >> 6;
+    const bool first_lane = (threadIdx.x & 63) == 0;
+    const int32_t *const index = in.index + row * in.k;
+    const float *const teacher = in.teacher + row * in.k;
+    bool bad = false, any = false, repeated = false;
+    float t_largest = -kInfinity;
     for (uint32_t e = threadIdx.x; e < in.k; e += THREADS) {
         const int32_t i = index[e];
         const float t = teacher[e];
-        const bool inside = i >= 0 && i < in.num_col;
-        if (!inside && i != -1) s.bad = 1;
-        const bool entry = inside && !(t == -kInfinity);
+        const bool inside = i >= 0 && i < in.num_col, entry = inside && !(t == -kInfinity);
+        bad |= !inside && i != -1;
+        any |= entry;
         s.index[e] = entry ? i : -1;
         s.q[e] = t;
-        if (entry) largest = fmaxf(largest, t), s.any = 1;
+        if (entry) t_largest = fmaxf(t_largest, t);
     }
-    float mt, lt, inverse = 1;
-    if (in.teacher_stats) {
-        mt = in.teacher_stats[2 * row], lt = in.teacher_stats[2 * row + 1];
-    } else {
-        mt = reference_of(block_max<THREADS>(largest, s.reduce));
-        float sum = 0;
-        for (uint32_t e = threadIdx.x; e < in.k; e += THREADS)
-            if (s.index[e] >= 0) sum += expf((s.q[e] - mt) / in.temperature);
-        sum = block_sum<THREADS>(sum, s.reduce);
-        lt = logf(sum);
-        inverse = 1.0f / sum;
+    float mine = wave_max(largest());
+    t_largest = wave_max(t_largest);
+    bad = __any(bad), any = __any(any);
+    if (first_lane) s.largest[wave] = mine, s.listed[wave] = t_largest, s.bad[wave] = bad, s.any[wave] = any;
+    __syncthreads();
+    row_answer r;
+    r.m = s.largest[0], t_largest = s.listed[0];
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) {
+        r.m = fmaxf(r.m, s.largest[w]), t_largest = fmaxf(t_largest, s.listed[w]);
+        bad |= s.bad[w] != 0, any |= s.any[w] != 0;
     }
-    float q = 0;
+    const float mt = in.teacher_stats ? in.teacher_stats[2 * row] : reference_of(t_largest);
+    float t_sum = 0;
+    for (uint32_t e = threadIdx.x; e < in.k; e += THREADS) {  // a thread's own entries
+        const int32_t i = s.index[e];
+        if (i < 0) continue;
+        repeated |= seen(i);
+        if (!in.teacher_stats) t_sum += expf((s.q[e] - mt) / in.temperature);
+    }
+    mine = wave_sum(sum(reference_of(r.m)));
+    t_sum = wave_sum(t_sum);
+    repeated = __any(repeated);
+    if (first_lane) s.sum[wave] = mine, s.listed_sum[wave] = t_sum, s.repeated[wave] = repeated;
+    __syncthreads();
+    r.sum = s.sum[0], t_sum = s.listed_sum[0];
+#pragma unroll
+    for (int w = 1; w < WAVES; w++) r.sum += s.sum[w], t_sum += s.listed_sum[w];
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) repeated |= s.repeated[w] != 0;
+    r.log_sum = logf(r.sum), r.repeated = repeated;
+    const float lt = in.teacher_stats ? in.teacher_stats[2 * row + 1] : logf(t_sum), inverse = 1.0f / t_sum;
+    float q_total = 0, loss = 0;
     for (uint32_t e = threadIdx.x; e < in.k; e += THREADS) {
-        float mine = 0;
-        if (s.index[e] >= 0) {
+        const int32_t i = s.index[e];
+        float q = 0;
+        if (i >= 0) {
             const float shifted = (s.q[e] - mt) / in.temperature;
-            mine = in.teacher_stats ? expf(shifted - lt) : expf(shifted) * inverse;
+            q = in.teacher_stats ? expf(shifted - lt) : expf(shifted) * inverse;
+            if (!(q == 0)) loss += q * ((shifted - lt) - ((logit(i) - r.m) / in.temperature - r.log_sum));  // 0 log 0 = 0
+            place(i, q);
         }
-        s.q[e] = mine;
-        q += mine;
+        s.q[e] = q;
+        q_total += q;
     }
-    q = block_sum<THREADS>(q, s.reduce);
-    *log_total = lt, *reference = mt;
-    return s.bad ? __builtin_nanf("") : q;
+    q_total = wave_sum(q_total), loss = wave_sum(loss);
+    if (first_lane) s.q_total[wave] = q_total, s.loss[wave] = loss;
+    __syncthreads();
+    r.q_total = s.q_total[0], r.loss = s.loss[0];
+#pragma unroll
+    for (int w = 1; w < WAVES; w++) r.q_total += s.q_total[w], r.loss += s.loss[w];
+    r.nothing = !bad && (!any || (r.m == -kInfinity && r.sum == r.sum));
+    if (bad) r.q_total = r.loss = __builtin_nanf("");
+    if (r.nothing) r.loss = 0;
+    return r;
 }
 
-// the row's loss; logit(e) is the student's logit of entry e
-template<int THREADS, class Logit>
-__device__ __forceinline__ float list_loss(const distill_input &in, int64_t row, list_shared &s, float q_total, float log_total, float reference, float m,
-                                           float log_sum, Logit logit) {
-    const float *teacher = in.teacher + row * in.k;
-    float sum = 0;
-    for (uint32_t e = threadIdx.x; e < in.k; e += THREADS) {
-        const float q = s.q[e];
-        if (s.index[e] < 0 || q == 0) continue;  // 0 log 0 = 0
-        const float log_q = (teacher[e] - reference) / in.temperature - log_total;
-        const float log_p = (logit(e) - m) / in.temperature - log_sum;
-        sum += q * (log_q - log_p);
+// Where a candidate is listed more than once: the sum of its entries' q to the first of them, in the list's order, so that the answer is
+// the same every time.  write(e, i, q): q for the first, the others get none.
+template<int THREADS, class Write>
+__device__ __forceinline__ void join_repeated(uint32_t k, const list_shared<THREADS> &s, Write write) {
+    for (uint32_t e = threadIdx.x; e < k; e += THREADS) {
+        const int32_t i = s.index[e];
+        if (i < 0) continue;
+        bool first = true;
+        float q = s.q[e];
+        for (uint32_t other = 0; other < k; other++) {
+            if (s.index[other] != i) continue;
+            if (other < e) first = false;
+            if (other > e) q += s.q[other];
+        }
+        if (first) write(e, i, q);
     }
-    sum = block_sum<THREADS>(sum, s.reduce);
-    if (q_total != q_total) return q_total;
-    return m == -kInfinity && log_sum == log_sum ? 0.0f : sum;
 }
 
-// What the gradient of elements [begin, begin + SIZE) takes from the list: a bit per element that has an entry, and there the
-// sum of its entries' q (in the list's order, so that an index that occurs twice gives the same answer every time).
+// What the gradient of a stretch of elements takes from the list: a bit per element that has a share, and there the share.
 template<int SIZE>
 struct listed_slice {
     uint32_t bits[SIZE / 32 + 1];
     float q[SIZE];
 };
 
-template<int THREADS, int SIZE>
-__device__ __forceinline__ void mark_listed(const distill_input &in, const list_shared &s, int64_t begin, listed_slice<SIZE> &l) {
-    for (int i = threadIdx.x; i < SIZE / 32 + 1; i += THREADS) l.bits[i] = 0;
-    __syncthreads();
-    for (uint32_t e = threadIdx.x; e < in.k; e += THREADS) {
-        const int32_t i = s.index[e];
-        if (i < begin || i >= begin + SIZE) continue;
-        bool first = true;
-        float q = s.q[e];
-        for (uint32_t other = 0; other < in.k; other++) {
-            if (s.index[other] != i) continue;
-            if (other < e) first = false;
-            if (other > e) q += s.q[other];
-        }
-        if (!first) continue;
-        l.q[i - begin] = q;
-        atomicOr(&l.bits[(i - begin) >> 5], 1u << ((i - begin) & 31));
-    }
-    __syncthreads();
-}
-
-// Nothing to learn from a row without entries, whatever its logits hold, nor from one whose candidates are all masked.
-__device__ __forceinline__ bool learns_nothing(const list_shared &s, float m, float sum) { return !s.bad && (!s.any || (m == -kInfinity && sum == sum)); }
-
-// gradient of a chunk: p_factor = w Q / (T S), q_factor = w / T
+// gradient of a chunk: p_factor = w Q / (T S), l.q times q_factor is subtracted
 template<class T, int SIZE>
 __device__ __forceinline__ void chunk_gradient(const uint4 raw, int place, float base, float scale, float p_factor, float q_factor, bool nothing,
                                                const listed_slice<SIZE> &l, float g[per_chunk<T>::value]) {
@@ -497,7 +520,7 @@ __device__ __forceinline__ void chunk_gradient(const uint4 raw, int place, float
     unpack<T>(raw, x);
 #pragma unroll
     for (int i = 0; i < E; i++) g[i] = nothing ? 0.0f : exp2_fast((x[i] - base) * scale) * p_factor;
-    // a chunk's place in the slice is a multiple of E, E divides 32: its bits lie in one word
+    // a chunk's place in the stretch is a multiple of E, E divides 32: its bits lie in one word
     const uint32_t mine = l.bits[place >> 5] >> (place & 31) & ((1u << E) - 1);
     if (mine && !nothing) {
 #pragma unroll
@@ -510,56 +533,73 @@ __device__ __forceinline__ void chunk_gradient(const uint4 raw, int place, float
 template<class T, int THREADS, int U, bool GRAD>
 __global__ void __launch_bounds__(THREADS) distill_row_kernel(distill_input in, distill_output out, int64_t first_row) {
     constexpr int E = per_chunk<T>::value, SIZE = THREADS * U * E;
-    __shared__ list_shared s;
+    __shared__ list_shared<THREADS> s;
     __shared__ listed_slice<GRAD ? SIZE : 32> l;
     const int64_t row = first_row + blockIdx.x;
     const chunked_row<T> z((const T *)in.logits + row * in.stride, in.num_col);
     uint4 raw[U];
 #pragma unroll
     for (int u = 0; u < U; u++) raw[u] = z.load(u * THREADS + threadIdx.x);
-    float log_total, reference;
-    float q_total = load_list<THREADS>(in, row, s, &log_total, &reference);
-    float largest = -kInfinity;
+    if constexpr (GRAD)
+        for (int i = threadIdx.x; i < SIZE / 32 + 1; i += THREADS) l.bits[i] = 0;
+    const row_answer r = solve_row<THREADS>(
+        in, row, s,
+        [&] {
+            float largest = -kInfinity;
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        float x[E];
-        unpack<T>(raw[u], x);
+            for (int u = 0; u < U; u++) {
+                float x[E];
+                unpack<T>(raw[u], x);
 #pragma unroll
-        for (int i = 0; i < E; i++) largest = fmaxf(largest, x[i]);
-    }
-    const float m = block_max<THREADS>(largest, s.reduce), base = reference_of(m);
-    float sum = 0;
+                for (int i = 0; i < E; i++) largest = fmaxf(largest, x[i]);
+            }
+            return largest;
+        },
+        [&](float base) {
+            float sum = 0;
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-        float x[E];
-        unpack<T>(raw[u], x);
+            for (int u = 0; u < U; u++) {
+                float x[E];
+                unpack<T>(raw[u], x);
 #pragma unroll
-        for (int i = 0; i < E; i++) sum += exp2_fast((x[i] - base) * in.scale);
-    }
-    sum = block_sum<THREADS>(sum, s.reduce);
-    const float log_sum = logf(sum);
-    const float loss = list_loss<THREADS>(in, row, s, q_total, log_total, reference, m, log_sum, [&](uint32_t e) { return to_float(z.row[s.index[e]]); });
+                for (int i = 0; i < E; i++) sum += exp2_fast((x[i] - base) * in.scale);
+            }
+            return sum;
+        },
+        [&](int32_t i) {
+            if constexpr (!GRAD) return false;
+            const int at = i + z.lead;
+            const uint32_t bit = 1u << (at & 31);
+            return (atomicOr(&l.bits[at >> 5], bit) & bit) != 0;
+        },
+        [&](int32_t i) { return to_float(z.row[i]); },
+        [&](int32_t i, float q) {
+            if constexpr (GRAD) l.q[i + z.lead] = q;
+        });
     if (threadIdx.x == 0) {
-        out.loss[row] = loss;
-        out.stats[2 * row] = m, out.stats[2 * row + 1] = log_sum;
+        out.loss[row] = r.loss;
+        out.stats[2 * row] = r.m, out.stats[2 * row + 1] = r.log_sum;
     }
     if constexpr (GRAD) {
-        const float q_factor = (in.weight ? in.weight[row] : 1.0f) / in.temperature;
-        const bool nothing = learns_nothing(s, m, sum);
-        const float p_factor = q_factor * q_total / sum;
-        mark_listed<THREADS, SIZE>(in, s, -z.lead, l);
+        if (r.repeated) {
+            join_repeated(in.k, s, [&](uint32_t, int32_t i, float q) { l.q[i + z.lead] = q; });
+            __syncthreads();
+        }
+        const float base = reference_of(r.m), q_factor = (in.weight ? in.weight[row] : 1.0f) / in.temperature, p_factor = q_factor * r.q_total / r.sum;
         T *grad = (T *)out.grad + row * out.grad_stride;
         const bool wide = (uintptr_t)grad % 16 == (uintptr_t)z.row % 16;
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int place = (u * THREADS + (int)threadIdx.x) * E;
             float g[E];
-            chunk_gradient<T, SIZE>(raw[u], place, base, in.scale, p_factor, q_factor, nothing, l, g);
+            chunk_gradient<T, SIZE>(raw[u], place, base, in.scale, p_factor, q_factor, r.nothing, l, g);
             store_chunk<T>(grad, (int64_t)place - z.lead, in.num_col, wide, g);
         }
     }
 }
 
+// Longer rows, in slices: max and sum of every slice; then, a workgroup per row, those joined and the list; then the gradient of every
+// slice, with nothing left to do per row but to find the slice's entries.
 constexpr int kSliceThreads = 256, kSliceElements = 8192;
 
 template<class T>
@@ -567,7 +607,6 @@ constexpr int slice_chunks() {
     return kSliceElements / kSliceThreads / per_chunk<T>::value;
 }
 
-// longer rows, first launch: max and sum of a slice, and the student's logits of the list's entries in it
 template<class T>
 __global__ void __launch_bounds__(kSliceThreads) distill_partial_kernel(distill_input in, distill_output out, int64_t first_row, uint32_t slices) {
     constexpr int E = per_chunk<T>::value, U = slice_chunks<T>();
@@ -578,13 +617,6 @@ __global__ void __launch_bounds__(kSliceThreads) distill_partial_kernel(distill_
     uint4 raw[U];
 #pragma unroll
     for (int u = 0; u < U; u++) raw[u] = z.load((int64_t)(slice * (uint64_t)U + u) * kSliceThreads + threadIdx.x);
-    if (out.listed) {
-        const int64_t begin = z.first((int64_t)slice * (U * kSliceThreads));
-        for (uint32_t e = threadIdx.x; e < in.k; e += kSliceThreads) {
-            const int64_t i = in.index[row * in.k + e];
-            if (i >= 0 && i < in.num_col && i >= begin && i < begin + kSliceElements) out.listed[(uint64_t)(blockIdx.x / slices) * in.k + e] = to_float(z.row[i]);
-        }
-    }
     float largest = -kInfinity;
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -606,81 +638,86 @@ __global__ void __launch_bounds__(kSliceThreads) distill_partial_kernel(distill_
     if (threadIdx.x == 0) out.partial[blockIdx.x] = make_float2(m, sum);
 }
 
-// max and sum of a row from those of its slices
-template<int THREADS>
-__device__ __forceinline__ void join_slices(const float2 *partial, uint32_t slices, float scale, float *shared, float *m_out, float *sum_out) {
-    float m = -kInfinity, sum = 0;
-    for (uint32_t i = threadIdx.x; i < slices; i += THREADS) m = fmaxf(m, partial[i].x);
-    m = block_max<THREADS>(m, shared);
-    const float base = reference_of(m);
-    for (uint32_t i = threadIdx.x; i < slices; i += THREADS) {
-        const float2 p = partial[i];
-        if (p.x > -kInfinity || p.y != p.y) sum += p.y * exp2_fast((reference_of(p.x) - base) * scale);
-    }
-    *sum_out = block_sum<THREADS>(sum, shared);
-    *m_out = m;
-}
+// Candidates of a list, hashed, to find out whether one is listed twice.
+constexpr uint32_t kSeen = 4 * kMaxList;
 
-// longer rows, the loss alone
-template<class T>
+template<class T, bool GIVEN>
 __global__ void __launch_bounds__(kSliceThreads) distill_finish_kernel(distill_input in, distill_output out, int64_t first_row, uint32_t slices) {
-    __shared__ list_shared s;
-    const int64_t row = first_row + blockIdx.x;
-    float log_total, reference, m, sum;
-    const float q_total = load_list<kSliceThreads>(in, row, s, &log_total, &reference);
-    join_slices<kSliceThreads>(out.partial + (uint64_t)blockIdx.x * slices, slices, in.scale, s.reduce, &m, &sum);
-    const float log_sum = logf(sum);
-    const T *z = (const T *)in.logits + row * in.stride;
-    const float loss = list_loss<kSliceThreads>(in, row, s, q_total, log_total, reference, m, log_sum, [&](uint32_t e) { return to_float(z[s.index[e]]); });
-    if (threadIdx.x == 0) {
-        out.loss[row] = loss;
-        out.stats[2 * row] = m, out.stats[2 * row + 1] = log_sum;
+    __shared__ list_shared<kSliceThreads> s;
+    __shared__ int32_t table[kSeen];
+    const int64_t row = first_row + blockIdx.x, local = blockIdx.x;
+    const float2 *const partial = out.partial + local * slices;
+    const T *const z = (const T *)in.logits + row * in.stride;
+    if (out.grad)
+        for (uint32_t i = threadIdx.x; i < kSeen; i += kSliceThreads) table[i] = -1;
+    const row_answer r = solve_row<kSliceThreads>(
+        in, row, s,
+        [&] {
+            if constexpr (GIVEN) return out.stats[2 * row];
+            float m = -kInfinity;
+            for (uint32_t i = threadIdx.x; i < slices; i += kSliceThreads) m = fmaxf(m, partial[i].x);
+            return m;
+        },
+        [&](float base) {
+            if constexpr (GIVEN) return threadIdx.x == 0 ? expf(out.stats[2 * row + 1]) : 0.0f;
+            float sum = 0;
+            for (uint32_t i = threadIdx.x; i < slices; i += kSliceThreads) {
+                const float2 p = partial[i];
+                if (p.x > -kInfinity || p.y != p.y) sum += p.y * exp2_fast((reference_of(p.x) - base) * in.scale);  // not a slice of nothing but masks
+            }
+            return sum;
+        },
+        [&](int32_t i) {
+            if (!out.grad) return false;
+            for (uint32_t at = (uint32_t)i * 2654435761u >> 20;; at++) {  // 12 bits; at most a quarter of the places are taken
+                const int32_t was = atomicCAS(&table[at % kSeen], -1, i);
+                if (was == -1) return false;
+                if (was == i) return true;
+            }
+        },
+        [&](int32_t i) { return GIVEN ? 0.0f : to_float(z[i]); }, [](int32_t, float) {});
+    if (!GIVEN && threadIdx.x == 0) {
+        out.loss[row] = r.loss;
+        out.stats[2 * row] = r.m, out.stats[2 * row + 1] = r.log_sum;
     }
+    if (!out.grad) return;
+    const float q_factor = (in.weight ? in.weight[row] : 1.0f) / in.temperature;
+    if (threadIdx.x == 0) out.factors[local] = make_float4(reference_of(r.m), q_factor * r.q_total / r.sum, 0.0f, r.nothing ? 1.0f : 0.0f);
+    int32_t *const index = out.index + local * in.k;
+    float *const q = out.q + local * in.k;
+    for (uint32_t e = threadIdx.x; e < in.k; e += kSliceThreads) index[e] = r.repeated ? -1 : s.index[e], q[e] = s.q[e] * q_factor;
+    if (r.repeated) join_repeated(in.k, s, [&](uint32_t e, int32_t i, float sum) { index[e] = i, q[e] = sum * q_factor; });  // a thread's own entries again
 }
 
-// the gradient of a slice; with LOSS the statistics come from the partial results and slice 0 writes the row's loss, else they are given
-template<class T, bool LOSS>
+template<class T>
 __global__ void __launch_bounds__(kSliceThreads) distill_grad_kernel(distill_input in, distill_output out, int64_t first_row, uint32_t slices) {
     constexpr int E = per_chunk<T>::value, U = slice_chunks<T>();
-    __shared__ list_shared s;
     __shared__ listed_slice<kSliceElements> l;
-    const int64_t row = first_row + blockIdx.x / slices;
+    const int64_t local = blockIdx.x / slices, row = first_row + local;
     const uint32_t slice = blockIdx.x % slices;
     const chunked_row<T> z((const T *)in.logits + row * in.stride, in.num_col);
-    const int64_t chunk0 = (int64_t)slice * (U * kSliceThreads);
+    const int64_t chunk0 = (int64_t)slice * (U * kSliceThreads), begin = z.first(chunk0);
     uint4 raw[U];
 #pragma unroll
     for (int u = 0; u < U; u++) raw[u] = z.load(chunk0 + u * kSliceThreads + threadIdx.x);
-    float log_total, reference, m, sum;
-    const float q_total = load_list<kSliceThreads>(in, row, s, &log_total, &reference);
-    if constexpr (LOSS) {
-        const uint32_t local = blockIdx.x / slices;
-        join_slices<kSliceThreads>(out.partial + (uint64_t)local * slices, slices, in.scale, s.reduce, &m, &sum);
-        if (slice == 0) {
-            const float log_sum = logf(sum);
-            const float loss = list_loss<kSliceThreads>(in, row, s, q_total, log_total, reference, m, log_sum,
-                                                        [&](uint32_t e) { return out.listed[(uint64_t)local * in.k + e]; });
-            if (threadIdx.x == 0) {
-                out.loss[row] = loss;
-                out.stats[2 * row] = m, out.stats[2 * row + 1] = log_sum;
-            }
-        }
-    } else {
-        m = out.stats[2 * row];
-        sum = expf(out.stats[2 * row + 1]);
+    const float4 f = out.factors[local];
+    for (int i = threadIdx.x; i < kSliceElements / 32 + 1; i += kSliceThreads) l.bits[i] = 0;
+    __syncthreads();
+    for (uint32_t e = threadIdx.x; e < in.k; e += kSliceThreads) {
+        const int64_t at = out.index[local * in.k + e] - begin;
+        if (out.index[local * in.k + e] < 0 || at < 0 || at >= kSliceElements) continue;
+        l.q[at] = out.q[local * in.k + e];
+        atomicOr(&l.bits[at >> 5], 1u << (at & 31));
     }
-    const float base = reference_of(m), q_factor = (in.weight ? in.weight[row] : 1.0f) / in.temperature;
-    const bool nothing = learns_nothing(s, m, sum);
-    const float p_factor = q_factor * q_total / sum;
-    mark_listed<kSliceThreads, kSliceElements>(in, s, z.first(chunk0), l);
+    __syncthreads();
     T *grad = (T *)out.grad + row * out.grad_stride;
     const bool wide = (uintptr_t)grad % 16 == (uintptr_t)z.row % 16;
 #pragma unroll
     for (int u = 0; u < U; u++) {
         const int place = (u * kSliceThreads + (int)threadIdx.x) * E;
         float g[E];
-        chunk_gradient<T, kSliceElements>(raw[u], place, base, in.scale, p_factor, q_factor, nothing, l, g);
-        store_chunk<T>(grad, z.first(chunk0) + place, in.num_col, wide, g);
+        chunk_gradient<T, kSliceElements>(raw[u], place, f.x, in.scale, f.y, 1.0f, f.w != 0, l, g);
+        store_chunk<T>(grad, begin + place, in.num_col, wide, g);
     }
 }
 
@@ -769,26 +806,44 @@ void launch_rows(hipStream_t stream, const distill_input &in, const distill_outp
 #undef GVK_ROWS
 }
 
+// bytes of a row's workspace: factors first, so that every part is aligned whatever the number of slices and entries
+size_t distill_row_bytes(int64_t slices, int k) { return sizeof(float4) + (size_t)slices * sizeof(float2) + (size_t)k * (sizeof(int32_t) + sizeof(float)); }
+
 template<class T>
-void launch_distill(hipStream_t stream, const distill_input &in, distill_output out, int64_t num_row, int64_t slices, bool one) {
-    const int64_t step = one ? kMaxGroups : (kMaxGroups / slices > 0 ? kMaxGroups / slices : 1);
-    const bool loss = out.loss != nullptr;
-    const distill_output all = out;
-    for (int64_t first = 0; first < num_row; first += step) {
-        const unsigned rows = (unsigned)(num_row - first < step ? num_row - first : step);
-        if (one) {
+void launch_distill(hipStream_t stream, const distill_input &in, distill_output out, int64_t num_row, int64_t slices, void *workspace) {
+    if (!workspace) {
+        for (int64_t first = 0; first < num_row; first += kMaxGroups) {
+            const unsigned rows = (unsigned)(num_row - first < kMaxGroups ? num_row - first : kMaxGroups);
             if (out.grad) launch_rows<T, true>(stream, in, out, first, rows);
             else launch_rows<T, false>(stream, in, out, first, rows);
-            continue;
         }
-        const dim3 grid(rows * (unsigned)slices), block(kSliceThreads);
-        if (all.partial) out.partial = all.partial + first * slices;
-        if (all.listed) out.listed = all.listed + first * in.k;
-        if (loss) hipLaunchKernelGGL((distill_partial_kernel<T>), grid, block, 0, stream, in, out, first, (uint32_t)slices);
-        if (!out.grad) hipLaunchKernelGGL((distill_finish_kernel<T>), dim3(rows), block, 0, stream, in, out, first, (uint32_t)slices);
-        else if (loss) hipLaunchKernelGGL((distill_grad_kernel<T, true>), grid, block, 0, stream, in, out, first, (uint32_t)slices);
-        else hipLaunchKernelGGL((distill_grad_kernel<T, false>), grid, block, 0, stream, in, out, first, (uint32_t)slices);
+        return;
     }
+    const int64_t step = kMaxGroups / slices > 0 ? kMaxGroups / slices : 1;
+    out.factors = (float4 *)workspace;
+    out.partial = (float2 *)(out.factors + num_row);
+    out.index = (int32_t *)(out.partial + num_row * slices);
+    out.q = (float *)(out.index + num_row * in.k);
+    const bool given = !out.loss;
+    for (int64_t first = 0; first < num_row; first += step) {
+        const unsigned rows = (unsigned)(num_row - first < step ? num_row - first : step);
+        const dim3 grid(rows * (unsigned)slices), block(kSliceThreads);
+        if (given) {
+            hipLaunchKernelGGL((distill_finish_kernel<T, true>), dim3(rows), block, 0, stream, in, out, first, (uint32_t)slices);
+        } else {
+            hipLaunchKernelGGL((distill_partial_kernel<T>), grid, block, 0, stream, in, out, first, (uint32_t)slices);
+            hipLaunchKernelGGL((distill_finish_kernel<T, false>), dim3(rows), block, 0, stream, in, out, first, (uint32_t)slices);
+        }
+        if (out.grad) hipLaunchKernelGGL((distill_grad_kernel<T>), grid, block, 0, stream, in, out, first, (uint32_t)slices);
+    }
+}
+
+int launch_distill_of(const char *who, int dtype, hipStream_t stream, const distill_input &in, const distill_output &out, int64_t num_row, void *workspace) {
+    const int64_t slices = distill_slices(dtype, in.num_col);
+    if (dtype == GVK_F32) launch_distill<float>(stream, in, out, num_row, slices, workspace);
+    else if (dtype == GVK_BF16) launch_distill<__bf16>(stream, in, out, num_row, slices, workspace);
+    else launch_distill<_Float16>(stream, in, out, num_row, slices, workspace);
+    return launched(who);
 }
 
 int check_distill(const char *who, int dtype, const void *logits, int64_t num_row, int64_t num_col, int64_t stride, int k, const int32_t *index,
@@ -853,7 +908,7 @@ extern "C" int gvk_top_logits(void *stream, int dtype, const void *logits, int64
 extern "C" size_t gvk_distill_workspace(int dtype, int64_t num_row, int64_t num_col, int k) {
     if ((dtype != GVK_F32 && dtype != GVK_BF16 && dtype != GVK_F16) || num_row < 1 || num_col < 1 || num_col > 0x7fffffff || k < 1 || k > kMaxList) return 0;
     if (one_launch(dtype, num_col)) return 0;
-    return (size_t)num_row * ((size_t)distill_slices(dtype, num_col) * sizeof(float2) + (size_t)k * sizeof(float));
+    return (size_t)num_row * distill_row_bytes(distill_slices(dtype, num_col), k);
 }
 
 extern "C" int gvk_distill(void *stream, int dtype, const void *logits, int64_t num_row, int64_t num_col, int64_t stride, int k, const int32_t *index,
@@ -869,20 +924,18 @@ extern "C" int gvk_distill(void *stream, int dtype, const void *logits, int64_t 
     const size_t need = gvk_distill_workspace(dtype, num_row, num_col, k);
     if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
         return gvk_fail(GVK_EINVAL, "%s: needs a workspace of %zu bytes on a multiple of 16, %zu given", who, need, workspace ? workspace_bytes : (size_t)0);
-    const int64_t slices = distill_slices(dtype, num_col);
-    const distill_input in = {logits, stride, num_col, index, teacher, teacher_stats, weight, (uint32_t)k, temperature, scale};
-    distill_output out = {loss, stats, grad, grad_stride, nullptr, nullptr};
-    if (need) out.partial = (float2 *)workspace, out.listed = grad ? (float *)((float2 *)workspace + (size_t)num_row * slices) : nullptr;
-    const bool one = need == 0;
-    if (dtype == GVK_F32) launch_distill<float>((hipStream_t)stream, in, out, num_row, slices, one);
-    else if (dtype == GVK_BF16) launch_distill<__bf16>((hipStream_t)stream, in, out, num_row, slices, one);
-    else launch_distill<_Float16>((hipStream_t)stream, in, out, num_row, slices, one);
-    return launched(who);
+    return launch_distill_of(who, dtype, (hipStream_t)stream, {logits, stride, num_col, index, teacher, teacher_stats, weight, (uint32_t)k, temperature, scale},
+                             {loss, stats, grad, grad_stride, nullptr, nullptr, nullptr, nullptr}, num_row, need ? workspace : nullptr);
+}
+
+extern "C" size_t gvk_distill_grad_workspace(int dtype, int64_t num_row, int64_t num_col, int k) {
+    if ((dtype != GVK_F32 && dtype != GVK_BF16 && dtype != GVK_F16) || num_row < 1 || num_col < 1 || num_col > 0x7fffffff || k < 1 || k > kMaxList) return 0;
+    return (size_t)num_row * distill_row_bytes(distill_slices(dtype, num_col), k);
 }
 
 extern "C" int gvk_distill_grad(void *stream, int dtype, const void *logits, int64_t num_row, int64_t num_col, int64_t stride, int k, const int32_t *index,
                                 const float *teacher, const float *teacher_stats, float temperature, const float *weight, const float *stats, void *grad,
-                                int64_t grad_stride) {
+                                int64_t grad_stride, void *workspace, size_t workspace_bytes) {
     const char *who = "gvk_distill_grad";
     int rc = check_distill(who, dtype, logits, num_row, num_col, stride, k, index, teacher, stats, grad, grad_stride);
     if (rc != GVK_OK) return rc;
@@ -890,11 +943,9 @@ extern "C" int gvk_distill_grad(void *stream, int dtype, const void *logits, int
     if ((rc = check_temperature(who, temperature, &scale)) != GVK_OK) return rc;
     if (num_row == 0) return GVK_OK;
     if (!grad) return gvk_fail(GVK_EINVAL, "%s: null pointer", who);
-    const distill_input in = {logits, stride, num_col, index, teacher, teacher_stats, weight, (uint32_t)k, temperature, scale};
-    const distill_output out = {nullptr, const_cast<float *>(stats), grad, grad_stride, nullptr, nullptr};
-    const int64_t slices = distill_slices(dtype, num_col);
-    if (dtype == GVK_F32) launch_distill<float>((hipStream_t)stream, in, out, num_row, slices, false);
-    else if (dtype == GVK_BF16) launch_distill<__bf16>((hipStream_t)stream, in, out, num_row, slices, false);
-    else launch_distill<_Float16>((hipStream_t)stream, in, out, num_row, slices, false);
-    return launched(who);
+    const size_t need = gvk_distill_grad_workspace(dtype, num_row, num_col, k);
+    if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16)
+        return gvk_fail(GVK_EINVAL, "%s: needs a workspace of %zu bytes on a multiple of 16, %zu given", who, need, workspace ? workspace_bytes : (size_t)0);
+    return launch_distill_of(who, dtype, (hipStream_t)stream, {logits, stride, num_col, index, teacher, teacher_stats, weight, (uint32_t)k, temperature, scale},
+                             {nullptr, const_cast<float *>(stats), grad, grad_stride, nullptr, nullptr, nullptr, nullptr}, num_row, workspace);
 }

@@ -463,10 +463,13 @@ class HipKernels(object):
         dev, rows, k = self._distill_list(logits, index, teacher, teacher_stats, weight)
         _need_shape(stats, torch.float32, "stats", dev, (rows, 2))
         _need_rows(grad, "grad", dev, (logits.dtype,), logits.shape)
+        dtype = _ROW_TYPES[logits.dtype]
+        nbytes = self.lib.gvk_distill_grad_workspace(dtype, rows, logits.shape[1], k)
         with _on(dev):
-            rc = self.lib.gvk_distill_grad(self._stream(logits), _ROW_TYPES[logits.dtype], _ptr(logits), rows, logits.shape[1],
-                                           _row_stride(logits), k, _ptr(index), _ptr(teacher), _ptr(teacher_stats), temperature,
-                                           _ptr(weight), _ptr(stats), _ptr(grad), _row_stride(grad))
+            workspace = self._workspace(nbytes, dev)
+            rc = self.lib.gvk_distill_grad(self._stream(logits), dtype, _ptr(logits), rows, logits.shape[1], _row_stride(logits), k,
+                                           _ptr(index), _ptr(teacher), _ptr(teacher_stats), temperature, _ptr(weight), _ptr(stats),
+                                           _ptr(grad), _row_stride(grad), _ptr(workspace), nbytes)
         _lib.check(rc, "gvk_distill_grad")
         return grad
 

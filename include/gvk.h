@@ -493,9 +493,10 @@ int gvk_distill(void *stream, int dtype, const void *logits, int64_t num_row, in
                 const float *teacher_stats, float temperature, const float *weight, float *loss, float *stats, void *grad, int64_t grad_stride,
                 void *workspace, size_t workspace_bytes);
 /* the gradient alone, from the stats of a forward pass over the same logits */
+size_t gvk_distill_grad_workspace(int dtype, int64_t num_row, int64_t num_col, int k);
 int gvk_distill_grad(void *stream, int dtype, const void *logits, int64_t num_row, int64_t num_col, int64_t stride, int k, const int32_t *index,
                      const float *teacher, const float *teacher_stats, float temperature, const float *weight, const float *stats, void *grad,
-                     int64_t grad_stride);
+                     int64_t grad_stride, void *workspace, size_t workspace_bytes);
 
 /* Named host ranges for profilers (roctx; `rocprofv3 --marker-trace`): the scopes the reference times with its
  * USE_TIMER Timer (include/util/time.h:28-60, include/core/solver.h:622,645,1526-1552).  Nesting allowed, per thread. */

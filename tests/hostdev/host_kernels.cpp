@@ -449,6 +449,7 @@ int gvk_predict(void *, int dim, const float *vertex, const float *context, cons
 size_t gvk_block_logits_workspace(int64_t, int) { return 0; }
 size_t gvk_top_logits_workspace(int, int64_t, int64_t, int) { return 0; }
 size_t gvk_distill_workspace(int, int64_t, int64_t, int) { return 0; }
+size_t gvk_distill_grad_workspace(int, int64_t, int64_t, int) { return 0; }
 int gvk_block_quantize(void *, int, const void *, int64_t, int, int64_t, uint8_t *, int64_t, uint8_t *) {
     return gvk_fail(GVK_EHIP, "gvk_block_quantize: not part of the host build");
 }
@@ -466,7 +467,7 @@ int gvk_distill(void *, int, const void *, int64_t, int64_t, int64_t, int, const
     return gvk_fail(GVK_EHIP, "gvk_distill: not part of the host build");
 }
 int gvk_distill_grad(void *, int, const void *, int64_t, int64_t, int64_t, int, const int32_t *, const float *, const float *, float, const float *, const float *,
-                     void *, int64_t) {
+                     void *, int64_t, void *, size_t) {
     return gvk_fail(GVK_EHIP, "gvk_distill_grad: not part of the host build");
 }
 

@@ -114,10 +114,14 @@ def test_distill_refuses(lib):
     refused(lib, distill(n=20000, stride=20000), "workspace")
     refused(lib, distill(n=20000, stride=20000, space=P, nbytes=lib.gvk_distill_workspace(0, 2, 20000, 3) - 1), "workspace")
     assert distill(m=0) == 0
-    assert lib.gvk_distill_workspace(0, 2, 16000, 3) == 0 and lib.gvk_distill_workspace(0, 2, 20000, 3) == 2 * (3 * 8 + 3 * 4)
+    assert lib.gvk_distill_workspace(0, 2, 16000, 3) == 0 and lib.gvk_distill_workspace(0, 2, 20000, 3) == 2 * (16 + 3 * 8 + 3 * 8)
 
-    def grad(z=P, m=2, n=9, stride=9, k=3, index=P, teacher=P, temperature=1.0, stats=P, g=apart, gstride=9):
-        return lib.gvk_distill_grad(None, 0, z, m, n, stride, k, index, teacher, None, temperature, None, stats, g, gstride)
+    def grad(z=P, m=2, n=9, stride=9, k=3, index=P, teacher=P, temperature=1.0, stats=P, g=apart, gstride=9, space=P, nbytes=1 << 20):
+        return lib.gvk_distill_grad(None, 0, z, m, n, stride, k, index, teacher, None, temperature, None, stats, g, gstride, space, nbytes)
+    need = lib.gvk_distill_grad_workspace(0, 2, 9, 3)
+    assert need == 2 * (16 + 8 + 3 * 8)
+    refused(lib, grad(space=None), "workspace")
+    refused(lib, grad(nbytes=need - 1), "workspace")
     for name in ("z", "index", "teacher", "stats", "g"):
         refused(lib, grad(**{name: None}), "null")
     refused(lib, grad(temperature=-1.0), "temperature")
