@@ -385,14 +385,14 @@ struct distill_output {
     int64_t grad_stride;
     // workspace of rows longer than a workgroup holds
     float2 *partial;   // [rows][slices]: max and sum
-    float4 *factors;   // [rows]: what the exponent subtracts, w Q / (T S), 0 or NaN to add, and whether there is nothing to learn
+    float4 *factors;   // [rows]: what the exponent subtracts, w Q / (T S), unused, 1 where there is nothing to learn
     int32_t *index;    // [rows][k]: candidates with a share of q, each once; -1: none
     float *q;          // [rows][k]: w q / T
 };
 
 template<int THREADS>
 struct list_shared {
-    int32_t index[kMaxList];  // -1 where the list has no entry
+    alignas(16) int32_t index[kMaxList];  // -1 where the list has no entry
     float q[kMaxList];        // first the logits, then the probabilities
     float largest[THREADS / 64], listed[THREADS / 64], sum[THREADS / 64], listed_sum[THREADS / 64], q_total[THREADS / 64], loss[THREADS / 64];
     uint32_t bad[THREADS / 64], any[THREADS / 64], repeated[THREADS / 64];
@@ -495,37 +495,43 @@ __device__ __forceinline__ void join_repeated(uint32_t k, const list_shared<THRE
         if (i < 0) continue;
         bool first = true;
         float q = s.q[e];
-        for (uint32_t other = 0; other < k; other++) {
-            if (s.index[other] != i) continue;
-            if (other < e) first = false;
-            if (other > e) q += s.q[other];
+        for (uint32_t at = 0; at < k; at += 4) {
+            const int4 four = *reinterpret_cast<const int4 *>(s.index + at);
+            const int32_t index[4] = {four.x, four.y, four.z, four.w};
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                if (index[u] != i || at + u >= k) continue;
+                if (at + u < e) first = false;
+                if (at + u > e) q += s.q[at + u];
+            }
         }
         if (first) write(e, i, q);
     }
 }
 
-// What the gradient of a stretch of elements takes from the list: a bit per element that has a share, and there the share.
-template<int SIZE>
+// What the gradient of a stretch of elements takes from the list: a bit per element that has a share, and there the share, or which
+// entry of the list holds it.
+template<int SIZE, class Share>
 struct listed_slice {
     uint32_t bits[SIZE / 32 + 1];
-    float q[SIZE];
+    Share share[SIZE];
 };
 
-// gradient of a chunk: p_factor = w Q / (T S), l.q times q_factor is subtracted
-template<class T, int SIZE>
-__device__ __forceinline__ void chunk_gradient(const uint4 raw, int place, float base, float scale, float p_factor, float q_factor, bool nothing,
-                                               const listed_slice<SIZE> &l, float g[per_chunk<T>::value]) {
+// gradient of a chunk: p_factor = w Q / (T S); share(place) is subtracted where the list has one
+template<class T, class Share>
+__device__ __forceinline__ void chunk_gradient(const uint4 raw, int place, float base, float scale, float p_factor, bool nothing, const uint32_t *bits, Share share,
+                                               float g[per_chunk<T>::value]) {
     constexpr int E = per_chunk<T>::value;
     float x[E];
     unpack<T>(raw, x);
 #pragma unroll
     for (int i = 0; i < E; i++) g[i] = nothing ? 0.0f : exp2_fast((x[i] - base) * scale) * p_factor;
     // a chunk's place in the stretch is a multiple of E, E divides 32: its bits lie in one word
-    const uint32_t mine = l.bits[place >> 5] >> (place & 31) & ((1u << E) - 1);
+    const uint32_t mine = bits[place >> 5] >> (place & 31) & ((1u << E) - 1);
     if (mine && !nothing) {
 #pragma unroll
         for (int i = 0; i < E; i++)
-            if (mine >> i & 1) g[i] -= l.q[place + i] * q_factor;
+            if (mine >> i & 1) g[i] -= share(place + i);
     }
 }
 
@@ -534,7 +540,7 @@ template<class T, int THREADS, int U, bool GRAD>
 __global__ void __launch_bounds__(THREADS) distill_row_kernel(distill_input in, distill_output out, int64_t first_row) {
     constexpr int E = per_chunk<T>::value, SIZE = THREADS * U * E;
     __shared__ list_shared<THREADS> s;
-    __shared__ listed_slice<GRAD ? SIZE : 32> l;
+    __shared__ listed_slice<GRAD ? SIZE : 32, float> l;
     const int64_t row = first_row + blockIdx.x;
     const chunked_row<T> z((const T *)in.logits + row * in.stride, in.num_col);
     uint4 raw[U];
@@ -574,7 +580,7 @@ __global__ void __launch_bounds__(THREADS) distill_row_kernel(distill_input in, 
         },
         [&](int32_t i) { return to_float(z.row[i]); },
         [&](int32_t i, float q) {
-            if constexpr (GRAD) l.q[i + z.lead] = q;
+            if constexpr (GRAD) l.share[i + z.lead] = q;
         });
     if (threadIdx.x == 0) {
         out.loss[row] = r.loss;
@@ -582,7 +588,7 @@ __global__ void __launch_bounds__(THREADS) distill_row_kernel(distill_input in, 
     }
     if constexpr (GRAD) {
         if (r.repeated) {
-            join_repeated(in.k, s, [&](uint32_t, int32_t i, float q) { l.q[i + z.lead] = q; });
+            join_repeated(in.k, s, [&](uint32_t, int32_t i, float q) { l.share[i + z.lead] = q; });
             __syncthreads();
         }
         const float base = reference_of(r.m), q_factor = (in.weight ? in.weight[row] : 1.0f) / in.temperature, p_factor = q_factor * r.q_total / r.sum;
@@ -592,7 +598,7 @@ __global__ void __launch_bounds__(THREADS) distill_row_kernel(distill_input in, 
         for (int u = 0; u < U; u++) {
             const int place = (u * THREADS + (int)threadIdx.x) * E;
             float g[E];
-            chunk_gradient<T, SIZE>(raw[u], place, base, in.scale, p_factor, q_factor, r.nothing, l, g);
+            chunk_gradient<T>(raw[u], place, base, in.scale, p_factor, r.nothing, l.bits, [&](int at) { return l.share[at] * q_factor; }, g);
             store_chunk<T>(grad, (int64_t)place - z.lead, in.num_col, wide, g);
         }
     }
@@ -692,7 +698,7 @@ __global__ void __launch_bounds__(kSliceThreads) distill_finish_kernel(distill_i
 template<class T>
 __global__ void __launch_bounds__(kSliceThreads) distill_grad_kernel(distill_input in, distill_output out, int64_t first_row, uint32_t slices) {
     constexpr int E = per_chunk<T>::value, U = slice_chunks<T>();
-    __shared__ listed_slice<kSliceElements> l;
+    __shared__ listed_slice<kSliceElements, uint16_t> l;
     const int64_t local = blockIdx.x / slices, row = first_row + local;
     const uint32_t slice = blockIdx.x % slices;
     const chunked_row<T> z((const T *)in.logits + row * in.stride, in.num_col);
@@ -706,7 +712,7 @@ __global__ void __launch_bounds__(kSliceThreads) distill_grad_kernel(distill_inp
     for (uint32_t e = threadIdx.x; e < in.k; e += kSliceThreads) {
         const int64_t at = out.index[local * in.k + e] - begin;
         if (out.index[local * in.k + e] < 0 || at < 0 || at >= kSliceElements) continue;
-        l.q[at] = out.q[local * in.k + e];
+        l.share[at] = (uint16_t)e;
         atomicOr(&l.bits[at >> 5], 1u << (at & 31));
     }
     __syncthreads();
@@ -716,7 +722,7 @@ __global__ void __launch_bounds__(kSliceThreads) distill_grad_kernel(distill_inp
     for (int u = 0; u < U; u++) {
         const int place = (u * kSliceThreads + (int)threadIdx.x) * E;
         float g[E];
-        chunk_gradient<T, kSliceElements>(raw[u], place, f.x, in.scale, f.y, 1.0f, f.w != 0, l, g);
+        chunk_gradient<T>(raw[u], place, f.x, in.scale, f.y, f.w != 0, l.bits, [&](int at) { return out.q[local * in.k + l.share[at]]; }, g);
         store_chunk<T>(grad, begin + place, in.num_col, wide, g);
     }
 }

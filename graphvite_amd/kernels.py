@@ -92,29 +92,48 @@ _ROW_TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16:
 
 
 def _need_rows(t, name, device=None, dtypes=_ROW_TYPES, shape=None):
-    """A 2-D GPU tensor whose rows are contiguous (any row stride that keeps them apart)."""
+    """A 2-D GPU tensor whose rows are contiguous (any row stride that keeps them apart): (address, rows, columns, row stride)."""
     if not isinstance(t, torch.Tensor) or t.dtype not in dtypes or t.dim() != 2:
         raise ValueError("%s must be a two-dimensional torch tensor of dtype %s" % (name, " or ".join(str(d) for d in dtypes)))
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    rows, columns = t.shape
+    if shape is not None and (rows, columns) != shape:
         raise ValueError("%s has shape %s, expected %s" % (name, tuple(t.shape), tuple(shape)))
-    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+    stride, step = t.stride()
+    if columns > 1 and step != 1 or rows > 1 and stride < columns:
         raise ValueError("the rows of %s must be contiguous and must not overlap (strides %s)" % (name, t.stride()))
-    if device is not None and t.device != device:
+    if device is None:
+        if not t.is_cuda:
+            raise ValueError("%s must live in GPU memory; graphvite_amd has no CPU path for it" % name)
+    elif t.device != device:
         raise ValueError("%s lives on %s, expected %s" % (name, t.device, device))
-    if not t.is_cuda:
-        raise ValueError("%s must live in GPU memory; graphvite_amd has no CPU path for it" % name)
-    return t
-
-
-def _row_stride(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return t.data_ptr(), rows, columns, stride if rows > 1 else columns
 
 
 def _need_shape(t, dtype, name, device, shape):
-    _need(t, dtype, name, device)
-    if tuple(t.shape) != tuple(shape):
+    """The address of a contiguous tensor of that shape; None for None."""
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or not t.is_contiguous():
+        raise ValueError("%s must be a contiguous torch tensor of dtype %s" % (name, dtype))
+    if t.shape != shape:
         raise ValueError("%s has shape %s, expected %s" % (name, tuple(t.shape), tuple(shape)))
+    if t.device != device:
+        raise ValueError("%s lives on %s, expected %s" % (name, t.device, device))
+    return t.data_ptr()
+
+
+def _need_tensor(t, name):
+    if not isinstance(t, torch.Tensor):
+        raise ValueError("%s must be a torch tensor" % name)
     return t
+
+
+def _current_stream(index):
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# the same number without a Stream object around it: 0.1 us against 2.8, where a whole call takes 8
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _current_stream)
 
 
 class BlockTable(object):
@@ -134,46 +153,19 @@ class BlockTable(object):
         dim = int(dim)
         if not 1 <= dim <= _lib.MAX_BLOCK_DIM:
             raise ValueError("dim must be 1 to %d, not %d" % (_lib.MAX_BLOCK_DIM, dim))
-        _need_rows(values, "values", None, (torch.uint8, torch.float8_e4m3fn))
-        _need_shape(exponents, torch.uint8, "exponents", values.device, (values.shape[0], (dim + 127) // 128))
-        if values.shape[1] < (dim + 15) // 16 * 16 or values.data_ptr() % 16 or values.shape[0] > 1 and values.stride(0) % 16:
+        address, self.rows, columns, stride = _need_rows(values, "values", None, (torch.uint8, torch.float8_e4m3fn))
+        self.device = values.device
+        _need_shape(exponents, torch.uint8, "exponents", self.device, (self.rows, (dim + 127) // 128))
+        if columns < (dim + 15) // 16 * 16 or address % 16 or self.rows > 1 and stride % 16:
             raise ValueError("values must hold dim rounded up to 16 columns per row, and start and step by multiples of 16 bytes")
         self.values, self.exponents, self.dim = values, exponents, dim
+        self._stride = stride if self.rows > 1 else columns // 16 * 16
 
     @staticmethod
     def empty(rows, dim, device):
         """An uninitialised table for HipKernels.quantize_blocks to fill."""
         return BlockTable(torch.empty((rows, (int(dim) + 15) // 16 * 16), dtype=torch.uint8, device=device),
                           torch.empty((rows, (int(dim) + 127) // 128), dtype=torch.uint8, device=device), dim)
-
-    @property
-    def rows(self):
-        return self.values.shape[0]
-
-    @property
-    def device(self):
-        return self.values.device
-
-    @property
-    def _stride(self):
-        return self.values.stride(0) if self.rows > 1 else self.values.shape[1] // 16 * 16
-
-
-class _on(object):
-    """Launches go to the tensors' device, whichever is current."""
-
-    def __init__(self, device):
-        self.device = device
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.device.index:
-            torch.cuda.set_device(self.device)
-
-    def __exit__(self, *exc):
-        if self.before != self.device.index:
-            torch.cuda.set_device(self.before)
-        return False
 
 
 class HipKernels(object):
@@ -354,32 +346,39 @@ class HipKernels(object):
 
     # ------------------------------------------------------------------------------------------- whole rows of candidates
     @staticmethod
+    def _on(device, call, *args):
+        """call(stream, *args) on the current stream of `device`, whichever device is current."""
+        index = device.index
+        if index == torch.cuda.current_device():
+            return call(_current_stream(index), *args)
+        with torch.cuda.device(index):
+            return call(_current_stream(index), *args)
+
+    @staticmethod
     def _workspace(nbytes, device):
-        """Scratch of one call: torch's allocator hands it on once the current stream has passed the call (a captured graph
-        has its own)."""
+        """Scratch of one call: torch's allocator hands it on once the current stream of the device has passed the call (a captured
+        graph has its own)."""
         return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
     def quantize_blocks(self, rows, table=None):
         """Rows (float32, bfloat16 or float16 [n, dim]) -> BlockTable: e4m3 with a power-of-two scale per 128 columns of a
         row.  `table`: an existing one of that shape to overwrite."""
-        _need_rows(rows, "rows")
+        address, n, dim, stride = _need_rows(rows, "rows")
         if table is None:
-            table = BlockTable.empty(rows.shape[0], rows.shape[1], rows.device)
-        if not isinstance(table, BlockTable) or table.device != rows.device or (table.rows, table.dim) != tuple(rows.shape):
+            table = BlockTable.empty(n, dim, rows.device)
+        if not isinstance(table, BlockTable) or table.device != rows.device or (table.rows, table.dim) != (n, dim):
             raise ValueError("table must be a BlockTable of the rows' shape on their device")
-        with _on(rows.device):
-            rc = self.lib.gvk_block_quantize(self._stream(rows), _ROW_TYPES[rows.dtype], _ptr(rows), rows.shape[0], rows.shape[1],
-                                             _row_stride(rows), _ptr(table.values), table._stride, _ptr(table.exponents))
-        _lib.check(rc, "gvk_block_quantize")
+        _lib.check(self._on(table.device, self.lib.gvk_block_quantize, _ROW_TYPES[rows.dtype], address, n, dim, stride,
+                            table.values.data_ptr(), table._stride, table.exponents.data_ptr()), "gvk_block_quantize")
         return table
 
     def dequantize_blocks(self, table, rows):
         """BlockTable -> rows (float32, bfloat16 or float16 [n, dim])."""
-        _need_rows(rows, "rows", table.device, shape=(table.rows, table.dim))
-        with _on(rows.device):
-            rc = self.lib.gvk_block_dequantize(self._stream(rows), _ptr(table.values), table._stride, _ptr(table.exponents), table.rows,
-                                               table.dim, _ROW_TYPES[rows.dtype], _ptr(rows), _row_stride(rows))
-        _lib.check(rc, "gvk_block_dequantize")
+        if not isinstance(table, BlockTable):
+            raise ValueError("table must be a BlockTable")
+        address, n, dim, stride = _need_rows(rows, "rows", table.device, shape=(table.rows, table.dim))
+        _lib.check(self._on(table.device, self.lib.gvk_block_dequantize, table.values.data_ptr(), table._stride,
+                            table.exponents.data_ptr(), n, dim, _ROW_TYPES[rows.dtype], address, stride), "gvk_block_dequantize")
         return rows
 
     def block_logits(self, query, table, logits):
@@ -387,54 +386,48 @@ class HipKernels(object):
         bfloat16 or float16.  Queries are quantised on the way in (blocks of 128 columns, as quantize_blocks)."""
         if not isinstance(table, BlockTable):
             raise ValueError("table must be a BlockTable")
-        dev = table.device
-        _need_rows(query, "query", dev)
-        _need_rows(logits, "logits", dev, shape=(query.shape[0], table.rows))
-        if query.shape[1] != table.dim:
-            raise ValueError("queries of %d columns against a table of %d" % (query.shape[1], table.dim))
-        nbytes = self.lib.gvk_block_logits_workspace(query.shape[0], table.dim)
-        with _on(dev):
-            workspace = self._workspace(nbytes, dev)
-            rc = self.lib.gvk_block_logits(self._stream(logits), _ROW_TYPES[query.dtype], _ptr(query), query.shape[0], _row_stride(query),
-                                           _ptr(table.values), table._stride, _ptr(table.exponents), table.rows, table.dim,
-                                           _ROW_TYPES[logits.dtype], _ptr(logits), _row_stride(logits), _ptr(workspace), nbytes)
-        _lib.check(rc, "gvk_block_logits")
+        device, dim = table.device, table.dim
+        q_address, m, columns, q_stride = _need_rows(query, "query", device)
+        z_address, _, n, z_stride = _need_rows(logits, "logits", device, shape=(m, table.rows))
+        if columns != dim:
+            raise ValueError("queries of %d columns against a table of %d" % (columns, dim))
+        nbytes = self.lib.gvk_block_logits_workspace(m, dim)
+        workspace = self._workspace(nbytes, device)
+        _lib.check(self._on(device, self.lib.gvk_block_logits, _ROW_TYPES[query.dtype], q_address, m, q_stride, table.values.data_ptr(),
+                            table._stride, table.exponents.data_ptr(), n, dim, _ROW_TYPES[logits.dtype], z_address, z_stride,
+                            workspace.data_ptr() if nbytes else None, nbytes), "gvk_block_logits")
         return logits
 
     def top_logits(self, logits, values, index, stats=None, temperature=1.0):
         """The k = values.shape[1] largest logits of each row: values float32 [m, k], largest first, of equal ones the lowest
         candidate; index int32 [m, k]; stats float32 [m, 2] = {max, log sum exp((logit - max) / temperature)}."""
-        dev = logits.device if isinstance(logits, torch.Tensor) else None
-        _need_rows(logits, "logits")
-        if not isinstance(values, torch.Tensor) or values.dim() != 2:
+        address, m, n, stride = _need_rows(logits, "logits")
+        device = logits.device
+        if _need_tensor(values, "values").dim() != 2:
             raise ValueError("values must be [rows, k]")
-        rows, k = logits.shape[0], values.shape[1]
-        _need_shape(values, torch.float32, "values", dev, (rows, k))
-        _need_shape(index, torch.int32, "index", dev, (rows, k))
-        if stats is not None:
-            _need_shape(stats, torch.float32, "stats", dev, (rows, 2))
+        k = values.shape[1]
+        v_address = _need_shape(values, torch.float32, "values", device, (m, k))
+        i_address = _need_shape(_need_tensor(index, "index"), torch.int32, "index", device, (m, k))
+        s_address = _need_shape(stats, torch.float32, "stats", device, (m, 2))
         dtype = _ROW_TYPES[logits.dtype]
-        nbytes = self.lib.gvk_top_logits_workspace(dtype, rows, logits.shape[1], k)
-        with _on(dev):
-            workspace = self._workspace(nbytes, dev)
-            rc = self.lib.gvk_top_logits(self._stream(logits), dtype, _ptr(logits), rows, logits.shape[1], _row_stride(logits), k,
-                                         temperature, _ptr(values), _ptr(index), _ptr(stats), _ptr(workspace), nbytes)
-        _lib.check(rc, "gvk_top_logits")
+        nbytes = self.lib.gvk_top_logits_workspace(dtype, m, n, k)
+        workspace = self._workspace(nbytes, device)
+        _lib.check(self._on(device, self.lib.gvk_top_logits, dtype, address, m, n, stride, k, temperature, v_address, i_address,
+                            s_address, workspace.data_ptr() if nbytes else None, nbytes), "gvk_top_logits")
         return values, index
 
     @staticmethod
-    def _distill_list(logits, index, teacher, teacher_stats, weight):
-        _need_rows(logits, "logits")
-        dev, rows = logits.device, logits.shape[0]
-        if not isinstance(index, torch.Tensor) or index.dim() != 2:
+    def _distill_input(logits, index, teacher, teacher_stats, temperature, weight):
+        """The arguments of gvk_distill and gvk_distill_grad up to the weight, the first of them the logits' type."""
+        address, m, n, stride = _need_rows(logits, "logits")
+        device = logits.device
+        if _need_tensor(index, "index").dim() != 2:
             raise ValueError("index must be [rows, k]")
-        _need_shape(index, torch.int32, "index", dev, (rows, index.shape[1]))
-        _need_shape(teacher, torch.float32, "teacher", dev, index.shape)
-        if teacher_stats is not None:
-            _need_shape(teacher_stats, torch.float32, "teacher_stats", dev, (rows, 2))
-        if weight is not None:
-            _need_shape(weight, torch.float32, "weight", dev, (rows,))
-        return dev, rows, index.shape[1]
+        k = index.shape[1]
+        return (_ROW_TYPES[logits.dtype], address, m, n, stride, k, _need_shape(index, torch.int32, "index", device, (m, k)),
+                _need_shape(_need_tensor(teacher, "teacher"), torch.float32, "teacher", device, (m, k)),
+                _need_shape(teacher_stats, torch.float32, "teacher_stats", device, (m, 2)), temperature,
+                _need_shape(weight, torch.float32, "weight", device, (m,)))
 
     def distill(self, logits, index, teacher, loss, stats, teacher_stats=None, temperature=1.0, weight=None, grad=None):
         """Kullback-Leibler divergence of softmax(logits / temperature) from a teacher's top logits, per row, and — with `grad` —
@@ -443,34 +436,31 @@ class HipKernels(object):
         index int32 [m, k]: candidates of the teacher's list (-1: no entry); teacher float32 [m, k]: their logits; teacher_stats
         float32 [m, 2] (top_logits of the teacher at the same temperature): probabilities of the teacher's whole row instead of the
         list's own; loss float32 [m], stats float32 [m, 2] are written; grad: like logits, may be logits itself."""
-        dev, rows, k = self._distill_list(logits, index, teacher, teacher_stats, weight)
-        _need_shape(loss, torch.float32, "loss", dev, (rows,))
-        _need_shape(stats, torch.float32, "stats", dev, (rows, 2))
+        given = self._distill_input(logits, index, teacher, teacher_stats, temperature, weight)
+        dtype, _, m, n, _, k = given[:6]
+        device = logits.device
+        loss_address = _need_shape(_need_tensor(loss, "loss"), torch.float32, "loss", device, (m,))
+        stats_address = _need_shape(_need_tensor(stats, "stats"), torch.float32, "stats", device, (m, 2))
+        g_address, g_stride = None, 0
         if grad is not None:
-            _need_rows(grad, "grad", dev, (logits.dtype,), logits.shape)
-        dtype = _ROW_TYPES[logits.dtype]
-        nbytes = self.lib.gvk_distill_workspace(dtype, rows, logits.shape[1], k)
-        with _on(dev):
-            workspace = self._workspace(nbytes, dev)
-            rc = self.lib.gvk_distill(self._stream(logits), dtype, _ptr(logits), rows, logits.shape[1], _row_stride(logits), k, _ptr(index),
-                                      _ptr(teacher), _ptr(teacher_stats), temperature, _ptr(weight), _ptr(loss), _ptr(stats), _ptr(grad),
-                                      0 if grad is None else _row_stride(grad), _ptr(workspace), nbytes)
-        _lib.check(rc, "gvk_distill")
+            g_address, _, _, g_stride = _need_rows(grad, "grad", device, (logits.dtype,), (m, n))
+        nbytes = self.lib.gvk_distill_workspace(dtype, m, n, k)
+        workspace = self._workspace(nbytes, device)
+        _lib.check(self._on(device, self.lib.gvk_distill, *given, loss_address, stats_address, g_address, g_stride,
+                            workspace.data_ptr() if nbytes else None, nbytes), "gvk_distill")
         return loss
 
     def distill_grad(self, logits, index, teacher, stats, grad, teacher_stats=None, temperature=1.0, weight=None):
         """The gradient of distill alone, from the stats that a forward pass over the same logits wrote."""
-        dev, rows, k = self._distill_list(logits, index, teacher, teacher_stats, weight)
-        _need_shape(stats, torch.float32, "stats", dev, (rows, 2))
-        _need_rows(grad, "grad", dev, (logits.dtype,), logits.shape)
-        dtype = _ROW_TYPES[logits.dtype]
-        nbytes = self.lib.gvk_distill_grad_workspace(dtype, rows, logits.shape[1], k)
-        with _on(dev):
-            workspace = self._workspace(nbytes, dev)
-            rc = self.lib.gvk_distill_grad(self._stream(logits), dtype, _ptr(logits), rows, logits.shape[1], _row_stride(logits), k,
-                                           _ptr(index), _ptr(teacher), _ptr(teacher_stats), temperature, _ptr(weight), _ptr(stats),
-                                           _ptr(grad), _row_stride(grad), _ptr(workspace), nbytes)
-        _lib.check(rc, "gvk_distill_grad")
+        given = self._distill_input(logits, index, teacher, teacher_stats, temperature, weight)
+        dtype, _, m, n, _, k = given[:6]
+        device = logits.device
+        stats_address = _need_shape(_need_tensor(stats, "stats"), torch.float32, "stats", device, (m, 2))
+        g_address, _, _, g_stride = _need_rows(grad, "grad", device, (logits.dtype,), (m, n))
+        nbytes = self.lib.gvk_distill_grad_workspace(dtype, m, n, k)
+        workspace = self._workspace(nbytes, device)
+        _lib.check(self._on(device, self.lib.gvk_distill_grad, *given, stats_address, g_address, g_stride,
+                            workspace.data_ptr() if nbytes else None, nbytes), "gvk_distill_grad")
         return grad
 
     def probe_row_traffic(self, vertex, context, pairs, negatives, bump=0.0):
