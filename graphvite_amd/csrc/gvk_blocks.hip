@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t *values, 
 // v_mfma_f32_16x16x32_bf16 with the TABLE as its first operand: a lane then ends with four consecutive candidates of one query
 // (n = 4 * (lane / 16) + r, m = lane % 16) and stores them at once.
 // Inside a block of 128 columns the order of the columns is free as long as both operands agree.  Lane group g = lane / 16 takes
-// columns j * 64 + g * 16 .. + 16 for j = 0, 1 — sixteen consecutive bytes of a table row, one load — and step s = 2 j + h of
+// columns j * 64 + g * 16 .. + 16 for j = 0, 1 — sixteen consecutive bytes of a table row — and step s = 2 j + h of
 // the four 32-column steps multiplies the half h of them.
 // Queries are laid out once as the fragments of that order: [block][16-row tile][step][lane][8] bf16, 4 KB per tile and block,
 // so that a wave reads a fragment as one contiguous KB, from LDS without bank conflicts.
@@ -246,26 +246,49 @@ struct table_view {
 // A wave's 64 rows of a table, four tiles of sixteen, as it walks along the columns.  Rows behind the last one are the last one (read, never
 // stored); columns behind a row's end are zero, by a mask after a load that stays inside the row: no branch, so that the
 // compiler counts the loads that are under way.
+// The matrix operand of a tile is 16 rows x 64 bytes; read as that, a load touches 16 cache lines by half and asks the L2 for each
+// twice.  So the two loads of a tile and block take whole lines, eight rows each: lane (r, g) of L0 holds row r % 8, sixteen bytes at
+// 16 g (r < 8) or 64 + 16 g (r >= 8), of L1 the same of row 8 + r % 8; halves of sixteen lanes change places (a DPP move) to make the
+// operands of it.  4096 x 65536 x d512: 409 -> 354 us, 4096 x 16384 x d4096: 618 -> 462 us, 64 x 1M x d512: 176 -> 154 us.
 struct table_rows {
-    const uint8_t *at[4], *exponent[4];
-    int padded, group;
+    const uint8_t *values, *exponents;  // of the strip's first row: the same for the wave
+    uint32_t at[4][2], exponent[4];
+    int padded, column;
 
-    __device__ __forceinline__ table_rows(const table_view &t, uint32_t first) : padded(t.padded), group((threadIdx.x & 63) >> 4) {
+    __device__ __forceinline__ table_rows(const table_view &t, uint32_t first) : padded(t.padded) {
+        const int lane = threadIdx.x & 63;
+        column = (lane >> 4) * 16 + (lane & 8) * 8;
+        first = __builtin_amdgcn_readfirstlane(first);
+        values = t.values + (int64_t)first * t.value_stride, exponents = t.exponents + (size_t)first * t.blocks;
+        const uint32_t last = t.num_row - 1 - first;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const uint32_t row = min(first + i * 16 + (threadIdx.x & 15), t.num_row - 1);
-            at[i] = t.values + (int64_t)row * t.value_stride;
-            exponent[i] = t.exponents + (size_t)row * t.blocks;
+            at[i][0] = min(i * 16u + (lane & 7), last) * (uint32_t)t.value_stride;
+            at[i][1] = min(i * 16u + 8 + (lane & 7), last) * (uint32_t)t.value_stride;
+            exponent[i] = min(i * 16u + (lane & 15), last) * t.blocks;
         }
     }
-    __device__ __forceinline__ uint4 load(int i, int block, int j) const {
-        const int column = block * kBlockColumns + j * 64 + group * 16;
-        const uint4 raw = *reinterpret_cast<const uint4 *>(at[i] + min(column, padded - 16));
-        const uint32_t mask = (uint32_t)((column - padded) >> 31);
+    // L0 or L1 of tile i
+    __device__ __forceinline__ uint4 load(int i, int block, int half) const {
+        const int c = block * kBlockColumns + column;
+        const uint4 raw = *reinterpret_cast<const uint4 *>(values + (at[i][half] + (uint32_t)min(c, padded - 16)));
+        const uint32_t mask = (uint32_t)((c - padded) >> 31);
         return uint4{raw.x & mask, raw.y & mask, raw.z & mask, raw.w & mask};
     }
-    __device__ __forceinline__ float scale(int i, int block) const { return __uint_as_float((uint32_t)exponent[i][block] << 23); }
+    __device__ __forceinline__ float scale(int i, int block) const { return __uint_as_float((uint32_t)exponents[exponent[i] + block] << 23); }
 };
+
+template<int BANKS>
+__device__ __forceinline__ uint32_t take_turned(uint32_t keep, uint32_t from) {  // lanes of BANKS take the lane eight places on in their sixteen
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)keep, (int)from, 0x128, 0xf, BANKS, false);
+}
+
+// L0, L1 -> columns 0 ... 63 and 64 ... 127 of the sixteen rows, lane (r, g) holding row r, sixteen bytes at 16 g
+__device__ __forceinline__ void change_places(uint4 &l0, uint4 &l1) {
+    const uint4 a = l0, b = l1;
+    l0 = uint4{take_turned<0xc>(a.x, b.x), take_turned<0xc>(a.y, b.y), take_turned<0xc>(a.z, b.z), take_turned<0xc>(a.w, b.w)};
+    l1 = uint4{take_turned<0x3>(b.x, a.x), take_turned<0x3>(b.y, a.y), take_turned<0x3>(b.z, a.z), take_turned<0x3>(b.w, a.w)};
+}
 
 // up to 16 queries: the table is read once and that bounds it.  Each workgroup lays the queries out for itself (no launch
 // before this one) and walks over strips of 64 candidates per wave.
@@ -292,6 +315,8 @@ __global__ void __launch_bounds__(256) few_queries_kernel(const Q *query, int64_
             float scale[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) raw[i][0] = rows.load(i, block, 0), raw[i][1] = rows.load(i, block, 1), scale[i] = rows.scale(i, block);
+#pragma unroll
+            for (int i = 0; i < 4; i++) change_places(raw[i][0], raw[i][1]);
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 bf16x8 b[2];
@@ -340,7 +365,9 @@ __global__ void __launch_bounds__(256, 3) narrow_kernel(const __bf16 *fragments,
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const float scale = rows.scale(i, 0);
-        widen(rows.load(i, 0, 0), scale, a[i]), widen(rows.load(i, 0, 1), scale, a[i] + 2);
+        uint4 l0 = rows.load(i, 0, 0), l1 = rows.load(i, 0, 1);
+        change_places(l0, l1);
+        widen(l0, scale, a[i]), widen(l1, scale, a[i] + 2);
     }
     const uint32_t begin = (uint32_t)((uint64_t)tiles * part / parts), end = (uint32_t)((uint64_t)tiles * (part + 1) / parts);
     const bf16x8 *const at = reinterpret_cast<const bf16x8 *>(fragments) + lane;
@@ -373,9 +400,13 @@ __global__ void __launch_bounds__(256, 2) logits_kernel(const __bf16 *fragments,
     constexpr int kTurns = 4 * (int)sizeof(wave_turn<T>) / 16;
     __shared__ uint4 even[TILES * 256 > kTurns ? TILES * 256 : kTurns], odd[TILES * 256];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t parts = (tiles + TILES - 1) / TILES;
+    // An XCD's workgroups take squares of up to 8 parts x 8 strips in turn, the strips first: its L2 holds what the 64 of them read.
+    const uint32_t parts = (tiles + TILES - 1) / TILES, strips = ((table.num_row + 255) / 256 + 7) / 8;  // strips of an XCD
     const uint32_t xcd = blockIdx.x % 8, turn = blockIdx.x / 8;
-    const uint32_t part = turn % parts, strip = (turn / parts) * 8 + xcd;
+    const uint32_t side = min(parts, 8u), column = turn / (side * strips), width = min(side, parts - column * side);
+    const uint32_t inside = turn - column * side * strips, row_group = inside / (width * 8), height = min(8u, strips - row_group * 8);
+    const uint32_t rest = inside - row_group * width * 8;
+    const uint32_t part = column * side + rest / height, strip = (row_group * 8 + rest % height) * 8 + xcd;
     if ((uint64_t)strip * 256 >= table.num_row) return;  // the whole workgroup
     const uint32_t first = strip * 256 + wave * 64, tile0 = part * TILES;
     f32x4 acc[TILES][4] = {};
@@ -398,24 +429,34 @@ __global__ void __launch_bounds__(256, 2) logits_kernel(const __bf16 *fragments,
         if (block + 1 < table.blocks) stage(other, block + 1);
         const int after = min(block + 1, table.blocks - 1);
         float next_scale[4];
+        // a fragment is asked for RING fragments before it is used: LDS answers meanwhile
+        constexpr int RING = 4;
+        bf16x8 ring[RING];
+        const auto fragment = [&](int t) {  // t = (step, tile)
+            return __builtin_bit_cast(bf16x8, staged[((t % TILES) * 4 + t / TILES) * 64 + lane]);
+        };
+#pragma unroll
+        for (int t = 0; t < RING && t < 4 * TILES; t++) ring[t] = fragment(t);
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             bf16x8 a[4][2];
 #pragma unroll
-            for (int i = 0; i < 4; i++) widen(raw[i][j], scale[i], a[i]);
+            for (int i = 0; i < 4; i++) {
+                if (j == 0) change_places(raw[i][0], raw[i][1]);
+                widen(raw[i][j], scale[i], a[i]);
+            }
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 raw[i][j] = rows.load(i, after, j);
                 if (j == 0) next_scale[i] = rows.scale(i, after);
             }
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
+            for (int t = 2 * j * TILES; t < 2 * (j + 1) * TILES; t++) {
 #pragma unroll
-                for (int tile = 0; tile < TILES; tile++) {
-                    const bf16x8 b = __builtin_bit_cast(bf16x8, staged[(tile * 4 + 2 * j + h) * 64 + lane]);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) acc[tile][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i][h], b, acc[tile][i], 0, 0, 0);
-                }
+                for (int i = 0; i < 4; i++) acc[t % TILES][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i][t / TILES - 2 * j], ring[t % RING], acc[t % TILES][i], 0, 0, 0);
+                if (t + RING < 4 * TILES) ring[t % RING] = fragment(t + RING);
+                __builtin_amdgcn_sched_group_barrier(0x8, 4, 0);    // four matrix instructions
+                __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // one read of LDS
             }
         }
 #pragma unroll
@@ -448,6 +489,7 @@ int check_rows(const char *who, int dtype, int64_t num_row, int dim, int64_t str
 int check_table(const char *who, const void *values, int64_t value_stride, const void *exponents, int dim) {
     if (!values || !exponents) return gvk_fail(GVK_EINVAL, "%s: null pointer", who);
     if (value_stride < (dim + 15) / 16 * 16) return gvk_fail(GVK_EINVAL, "%s: %d columns need a value stride of %d, not %lld", who, dim, (dim + 15) / 16 * 16, (long long)value_stride);
+    if (value_stride > GVK_MAX_BLOCK_STRIDE) return gvk_fail(GVK_EINVAL, "%s: a value stride of %lld", who, (long long)value_stride);
     if (!aligned(values, value_stride, 16)) return gvk_fail(GVK_EINVAL, "%s: values and their stride must be multiples of 16 bytes", who);
     return GVK_OK;
 }

@@ -442,6 +442,7 @@ int gvk_describe_train(int dim, int optimizer_type, int num_negative, int explic
 enum { GVK_F32 = 0, GVK_BF16 = 1, GVK_F16 = 2 };
 #define GVK_MAX_BLOCK_DIM 4096
 #define GVK_MAX_BLOCK_ROWS 0x7fffff00
+#define GVK_MAX_BLOCK_STRIDE (1 << 24) /* bytes from row to row of a table */
 #define GVK_MAX_BLOCK_QUERIES (1 << 20)
 #define GVK_MAX_TOP 256            /* entries gvk_top_logits gives per row */
 #define GVK_MAX_DISTILL_LIST 1024  /* entries of a teacher's list */
