@@ -249,7 +249,7 @@ struct table_view {
 // The matrix operand of a tile is 16 rows x 64 bytes; read as that, a load touches 16 cache lines by half and asks the L2 for each
 // twice.  So the two loads of a tile and block take whole lines, eight rows each: lane (r, g) of L0 holds row r % 8, sixteen bytes at
 // 16 g (r < 8) or 64 + 16 g (r >= 8), of L1 the same of row 8 + r % 8; halves of sixteen lanes change places (a DPP move) to make the
-// operands of it.  4096 x 65536 x d512: 409 -> 354 us, 4096 x 16384 x d4096: 618 -> 462 us, 64 x 1M x d512: 176 -> 154 us.
+// operands of it.  4096 x 65536 x d512, bf16: 388 -> 338 us together with the order of the workgroups, 1 x 1M x d512: 115 -> 102 us.
 struct table_rows {
     const uint8_t *values, *exponents;  // of the strip's first row: the same for the wave
     uint32_t at[4][2], exponent[4];
@@ -339,28 +339,37 @@ __global__ void __launch_bounds__(256) few_queries_kernel(const Q *query, int64_
     }
 }
 
-// up to 128 columns, 64 candidates and 17 queries or more: what moves is the answer, and the table once.  A wave widens 64 candidates into
+// up to 128 columns, 256 candidates and 17 queries or more: what moves is the answer, and the table once.  A wave widens 64 candidates into
 // registers and walks over the queries' tiles, whose fragments (4 KB each, the same for every wave) come through L1: sixteen matrix
-// instructions and 64 x 16 logits a step, no barrier.  Loads and stores of a wave come back in order, so what is loaded behind
-// stores waits until those are in memory: the next tile's fragments are asked for before this tile's logits are stored, and
-// nothing on the way is conditional, so that the wait is for the loads alone (the last tile and the last strip are moved back to
-// end with the rows: some logits are computed twice, to the same bits).
-// Measured at 1024 x 1M x d128: f32 835 us, bf16 478; without the table's loads 773 and 395, the stores alone 745 and 380, in any order
-// of them: the write rate of rows (5.5 TB/s) bounds it, and reads between the writes cost more than their bytes.  Three workgroups
-// to a CU (held by LDS they do not use): with four, the writes of more rows meet, 853 and 492; with two, 911 and 454.  Waves that stay
-// and walk over strips with the queries in LDS: 882 and 476.
-constexpr size_t kThreeToACu = 52 * 1024;
+// instructions and 64 x 16 logits a step; the four waves of a workgroup put theirs side by side in LDS and store 256 candidates of a row
+// at once.  Loads and stores of a wave come back in order, so what is loaded behind stores waits until those are in memory: the next
+// tile's fragments are asked for before this tile's logits are stored, and nothing on the way is conditional, so that the wait is for
+// the loads alone (the last tile and the last strip are moved back to end with the rows: some logits are computed twice, to the
+// same bits).
+// Rows that begin anywhere share cache lines with their neighbours' stores, and a line written in parts by two L2s, or twice by one, costs
+// memory a read as well: hence the wide stores, and an XCD takes an eighth of the candidates, in order, the parts of a strip one after
+// the other (777 x 99991 f16 on eight outputs in turn: 64 us with 64 candidates of a row at once and strips dealt over the XCDs, 49 with
+// the strips in order, 45 with 256 candidates; 777 x 99968, whose rows begin on lines: 40).
+// 1024 x 1M x d128: f32 817 us, bf16 440; without the table's loads 773 and 395, the stores alone 745 and 380 in any order of them: the write
+// rate of rows (5.5 TB/s) bounds it, and reads between the writes cost more than their bytes.  Waves that stay and walk over
+// strips with the queries in LDS: 882 and 476.
+// 16 queries x 256 candidates of a workgroup on their way from the waves' registers to memory
+template<class T>
+struct group_turn {
+    static constexpr int pitch = 256 * (int)sizeof(T) + 16;
+    uint4 bytes[2][16 * pitch / 16];
+};
 
 template<class T>
-__global__ void __launch_bounds__(256, 3) narrow_kernel(const __bf16 *fragments, uint32_t tiles, uint32_t num_query, uint32_t parts, table_view table, T *logits,
+__global__ void __launch_bounds__(256, 4) narrow_kernel(const __bf16 *fragments, uint32_t tiles, uint32_t num_query, uint32_t parts, table_view table, T *logits,
                                                         int64_t logit_stride) {
-    __shared__ wave_turn<T> turns[4];
+    __shared__ group_turn<T> turns;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t xcd = blockIdx.x % 8, turn = blockIdx.x / 8;  // the parts of a strip: consecutive on one XCD
-    const uint32_t part = turn % parts, strip = ((turn / parts) * 8 + xcd) * 4 + wave;
-    if ((uint64_t)strip * 64 >= table.num_row) return;
-    const uint32_t first = min(strip * 64, table.num_row - 64);
-    const table_rows rows(table, first);
+    const uint32_t xcd = blockIdx.x % 8, turn = blockIdx.x / 8;
+    const uint32_t part = turn % parts, strip = xcd * (gridDim.x / 8 / parts) + turn / parts;
+    if ((uint64_t)strip * 256 >= table.num_row) return;
+    const uint32_t first = min(strip * 256, table.num_row - 256);
+    const table_rows rows(table, first + wave * 64);
     bf16x8 a[4][4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -376,6 +385,7 @@ __global__ void __launch_bounds__(256, 3) narrow_kernel(const __bf16 *fragments,
 #pragma unroll
         for (int s = 0; s < 4; s++) b[s] = at[(size_t)(tile * 4 + s) * 64];
     };
+    constexpr int E = 16 / (int)sizeof(T), lanes = 256 / E, rows_at_once = 64 / lanes;  // lanes to a row, rows to an instruction of a wave
     fetch(begin);
     wait_for_loads();
     for (uint32_t tile = begin; tile < end; tile++) {
@@ -386,7 +396,20 @@ __global__ void __launch_bounds__(256, 3) narrow_kernel(const __bf16 *fragments,
             for (int i = 0; i < 4; i++) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i][s], b[s], acc[i], 0, 0, 0);
         }
         fetch(min(tile + 1, end - 1));
-        store_turned<true>(turns[wave], logits, logit_stride, min(tile * 16, num_query - 16), num_query, first, table.num_row, acc);
+        char *const bytes = reinterpret_cast<char *>(turns.bytes[tile & 1]);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            T t[4] = {from_float<T>(acc[i][0]), from_float<T>(acc[i][1]), from_float<T>(acc[i][2]), from_float<T>(acc[i][3])};
+            __builtin_memcpy(__builtin_assume_aligned(bytes + (lane & 15) * group_turn<T>::pitch + (wave * 64 + i * 16 + (lane >> 4) * 4) * (int)sizeof(T), 4 * sizeof(T)), t, sizeof(t));
+        }
+        __syncthreads();
+        const uint32_t m0 = min(tile * 16, num_query - 16);
+#pragma unroll
+        for (int i = 0; i < 4 / rows_at_once; i++) {
+            const int row = wave * 4 + i * rows_at_once + lane / lanes, column = lane % lanes * E;
+            const uint4 raw = *reinterpret_cast<const uint4 *>(bytes + row * group_turn<T>::pitch + column * (int)sizeof(T));
+            __builtin_memcpy(logits + (int64_t)(m0 + row) * logit_stride + first + column, &raw, 16);
+        }
     }
 }
 
@@ -406,7 +429,7 @@ __global__ void __launch_bounds__(256, 2) logits_kernel(const __bf16 *fragments,
     const uint32_t side = min(parts, 8u), column = turn / (side * strips), width = min(side, parts - column * side);
     const uint32_t inside = turn - column * side * strips, row_group = inside / (width * 8), height = min(8u, strips - row_group * 8);
     const uint32_t rest = inside - row_group * width * 8;
-    const uint32_t part = column * side + rest / height, strip = (row_group * 8 + rest % height) * 8 + xcd;
+    const uint32_t part = column * side + rest / height, strip = xcd * strips + row_group * 8 + rest % height;
     if ((uint64_t)strip * 256 >= table.num_row) return;  // the whole workgroup
     const uint32_t first = strip * 256 + wave * 64, tile0 = part * TILES;
     f32x4 acc[TILES][4] = {};
@@ -516,17 +539,22 @@ int launch_logits(hipStream_t stream, const Q *query, int64_t query_stride, uint
     }
     const uint32_t tiles = (num_query + 15) / 16;
     __bf16 *fragments = reinterpret_cast<__bf16 *>(workspace);
-    const bool narrow = table.blocks == 1 && num_query > 16 && table.num_row >= 64;
+    const bool narrow = table.blocks == 1 && num_query > 16 && table.num_row >= 256;
     hipLaunchKernelGGL((fragment_kernel<Q>), dim3((tiles * 16 * table.blocks + 7) / 8), dim3(256), 0, stream, query, query_stride, query_wide,
                        num_query, tiles, dim, table.blocks, narrow, fragments);
     const uint64_t strips = ((uint64_t)table.num_row + 255) / 256;
     if (narrow) {
-        // parts of at least eight tiles, until there are eight waves for every SIMD (777 x 99991: 40 us at six parts, 41.6 at four)
+        // The chip holds 1024 workgroups: as many parts as make the longest row of them on one place shortest, the table's rows counting as
+        // four tiles (777 x 99991: 391 strips x 5 parts of ten tiles, two in a row; 4 parts of thirteen: two in a row as well)
         uint32_t parts = 1;
-        while (strips * parts < 2048 && tiles / (parts * 2) >= 8) parts *= 2;
+        uint64_t least = ~0ull;
+        for (uint32_t p = 1; p <= tiles && p <= 64; p++) {
+            const uint64_t cost = ((strips + 7) / 8 * 8 * p + 1023) / 1024 * ((tiles + p - 1) / p + 4);
+            if (cost < least) least = cost, parts = p;
+        }
         const uint64_t grid = (strips + 7) / 8 * 8 * parts;
         if (grid > 0xffffffull) return gvk_fail(GVK_EINVAL, "gvk_block_logits: too many logits for one call");
-        hipLaunchKernelGGL((narrow_kernel<T>), dim3((unsigned)grid), dim3(256), kThreeToACu - 4 * sizeof(wave_turn<T>), stream, fragments, tiles, num_query, parts, table, logits, logit_stride);
+        hipLaunchKernelGGL((narrow_kernel<T>), dim3((unsigned)grid), dim3(256), 0, stream, fragments, tiles, num_query, parts, table, logits, logit_stride);
         return launched("gvk_block_logits");
     }
 #define GVK_LOGITS(TILES)                                                                                                                 \
