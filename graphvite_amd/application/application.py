@@ -328,6 +328,26 @@ class GraphApplication(ApplicationMixin):
         auc = float(hit[Y == 0].sum()) / total if total else float("nan")
         return {"AUC": auc}
 
+    def neighbor_prediction(self, H=None, file_name=None, k=10):
+        """
+        Predict the k most likely neighbors of each node: the nodes with the largest score = <vertex[h], context[t]> of all, scored with
+        the context table in 8 bits (GraphSolver.scorer).  The node-embedding counterpart of the reference's entity prediction.
+
+        Parameters:
+            H (list, optional): nodes
+            file_name (str, optional): file with one node per line
+            k (int): up to 256
+
+        Returns:
+            list of lists of (node, score), for each node the best first
+        """
+        if self.one_source((H,), file_name, "Node"):
+            (H,) = self.read_columns(file_name, 1, "node file")
+        ids = self.get_mapping([str(h) for h in H], self.graph.name2id)
+        index, scores, _ = self.solver.scorer().top(ids, k)
+        id2name = self.graph.id2name
+        return [[(id2name[int(t)], float(score)) for t, score in zip(*row)] for row in zip(index, scores)]
+
 
 def linear_classification(embeddings, labels, portion, normalization=False, times=1, patience=100):
     """One-vs-rest logistic regression on frozen embeddings, as the reference's linear_classification

@@ -1,0 +1,144 @@
+"""Answers of a trained model for whole rows of candidates, and learning from them.
+
+`GraphSolver.predict` gives the logits <vertex[h], context[t]> of given pairs.  A `LinkScorer` — made by `GraphSolver.scorer()` — gives a
+node's logits against EVERY node, or the best of them, from a context table held on the GPU in 8 bits
+(`HipKernels.quantize_blocks`): a quarter of the memory, and of the time where reading the table is what an answer costs.
+`distill` (as `GraphSolver.distill`) trains a solver's embeddings — of a smaller dimension, say — to answer as a scorer does.
+"""
+import numpy as np
+import torch
+
+from .kernels import HipKernels
+
+_CHUNK = 1 << 28  # logits of a batch: a float32 GiB
+
+
+def node_rows(heads, num_vertex, device):
+    """Node ids as an index tensor on `device`, checked on the host."""
+    heads = np.asarray(heads)
+    if heads.ndim != 1 or heads.dtype.kind not in "iu":
+        raise ValueError("Expect a one-dimensional array of node ids, but %s of shape %s is found" % (heads.dtype, heads.shape))
+    if len(heads) and (int(heads.min()) < 0 or int(heads.max()) >= num_vertex):
+        raise ValueError("node index out of range")
+    return torch.from_numpy(heads.astype(np.int64)).to(device)
+
+
+class LinkScorer(object):
+    """
+    LinkScorer(solver, device=None)
+    The embeddings of a built solver as they are now, ready to answer: vertex rows in float32, the context table in 8 bits with a
+    power-of-two scale per 128 columns, both on one GPU.  Later changes of the solver's embeddings do not show; make another.
+
+    Parameters:
+        solver (GraphSolver): built (and trained, or loaded) solver, no session open
+        device (int, optional): GPU id, default is the solver's first
+
+    Logits are off from `GraphSolver.predict` by the rounding to 8 bits on both sides: up to 2^-4 of each value.
+    """
+
+    def __init__(self, solver, device=None):
+        if solver.graph is None:
+            raise RuntimeError("The model must be built on a graph first")
+        solver._no_session("scorer")
+        self.device = torch.device("cuda", solver.device if device is None else int(device))
+        self.graph, self.dim, self.num_vertex = solver.graph, solver.dim, solver.num_vertex
+        self.kernels = HipKernels()
+        self.vertex = torch.from_numpy(solver.vertex_embeddings).to(self.device)
+        self.table = self.kernels.quantize_blocks(torch.from_numpy(solver.context_embeddings).to(self.device))
+
+    def logits(self, heads, dtype=torch.float32):
+        """
+        logits(heads, dtype=torch.float32)
+        Logits of nodes against all nodes.
+
+        Parameters:
+            heads (ndarray): node ids
+            dtype (torch.dtype): float32, bfloat16 or float16
+
+        Returns:
+            Tensor: [len(heads), num_vertex] on the scorer's GPU, ordered on its current stream
+        """
+        with torch.cuda.device(self.device):
+            rows = node_rows(heads, self.num_vertex, self.device)
+            out = torch.empty((len(rows), self.num_vertex), dtype=dtype, device=self.device)
+            return self.kernels.block_logits(self.vertex[rows], self.table, out)
+
+    def top_on_device(self, rows, k, temperature=1.0):
+        """(logits float32 [n, k], index int32 [n, k], stats float32 [n, 2]) of an index tensor on the scorer's GPU; HipKernels.top_logits."""
+        n, device = len(rows), self.device
+        values = torch.empty((n, k), dtype=torch.float32, device=device)
+        index = torch.empty((n, k), dtype=torch.int32, device=device)
+        stats = torch.empty((n, 2), dtype=torch.float32, device=device)
+        batch = max(1, min(n, _CHUNK // self.num_vertex))
+        logits = torch.empty((batch, self.num_vertex), dtype=torch.float32, device=device)
+        for first in range(0, n, batch):
+            part = rows[first:first + batch]
+            z = logits[:len(part)]
+            self.kernels.block_logits(self.vertex[part], self.table, z)
+            self.kernels.top_logits(z, values[first:first + batch], index[first:first + batch], stats[first:first + batch], temperature)
+        return values, index, stats
+
+    def top(self, heads, k=10, temperature=1.0):
+        """
+        top(heads, k=10, temperature=1.0)
+        The k nodes with the largest logits for each node, the largest first, of equal ones the lowest id.
+
+        Parameters:
+            heads (ndarray): node ids
+            k (int): up to 256, and no more than there are nodes
+            temperature (float): of the statistics
+
+        Returns:
+            (ndarray, ndarray, ndarray): ids int64 [n, k]; logits float32 [n, k]; float32 [n, 2] = max m and
+            log sum exp((logit - m) / temperature) of each whole row
+        """
+        if not 1 <= int(k) <= min(256, self.num_vertex):
+            raise ValueError("k must be 1 to %d, not %s" % (min(256, self.num_vertex), k))
+        with torch.cuda.device(self.device):
+            values, index, stats = self.top_on_device(node_rows(heads, self.num_vertex, self.device), int(k), float(temperature))
+            return index.cpu().numpy().astype(np.int64), values.cpu().numpy(), stats.cpu().numpy()
+
+
+def distill(solver, teacher, heads=None, num_epoch=1, batch_size=0, k=64, temperature=1.0, lr=0.025, seed=None):
+    """GraphSolver.distill."""
+    if solver.graph is None:
+        raise RuntimeError("The model must be built on a graph first")
+    solver._no_session("distill")
+    if not isinstance(teacher, LinkScorer):
+        raise TypeError("teacher must be a LinkScorer (GraphSolver.scorer() of the solver to learn from)")
+    if teacher.graph is not solver.graph and list(teacher.graph.id2name) != list(solver.graph.id2name):
+        raise ValueError("the teacher's nodes are not this solver's nodes")
+    n = solver.num_vertex
+    if not 1 <= int(k) <= min(256, n):
+        raise ValueError("k must be 1 to %d, not %s" % (min(256, n), k))
+    if int(num_epoch) < 0 or int(batch_size) < 0 or not lr > 0:
+        raise ValueError("num_epoch and batch_size must not be negative, and lr must be positive")
+    device, kernels = teacher.device, teacher.kernels
+    batch = int(batch_size) or max(1, min(1024, _CHUNK // n))
+    generator = torch.Generator()
+    generator.manual_seed(solver.seed if seed is None else int(seed))
+    with torch.cuda.device(device):
+        rows = node_rows(np.arange(n) if heads is None else heads, n, device)
+        if len(torch.unique(rows)) != len(rows):
+            raise ValueError("a node is named twice")  # its row would be written twice in a batch
+        values, index, teacher_stats = teacher.top_on_device(rows, int(k), float(temperature))
+        vertex = torch.from_numpy(solver.vertex_embeddings).to(device)
+        context = torch.from_numpy(solver.context_embeddings).to(device)
+        losses = []
+        for _ in range(int(num_epoch)):
+            total = torch.zeros((), dtype=torch.float64, device=device)
+            for part in torch.randperm(len(rows), generator=generator).to(device).split(batch):
+                ids = rows[part]
+                v = vertex[ids]
+                logits = v @ context.t()
+                loss = torch.empty(len(ids), device=device)
+                stats = torch.empty((len(ids), 2), device=device)
+                kernels.distill(logits, index[part], values[part], loss, stats, teacher_stats[part], float(temperature), grad=logits)
+                change = logits @ context  # before the context moves: both sides from what the batch began with
+                context.addmm_(logits.t(), v, alpha=-lr)
+                vertex[ids] = v - lr * change
+                total += loss.sum(dtype=torch.float64)
+            losses.append(float(total) / max(len(rows), 1))
+        solver.vertex_embeddings[:] = vertex.cpu().numpy()
+        solver.context_embeddings[:] = context.cpu().numpy()
+    return losses

@@ -115,7 +115,7 @@ class TrainingSession(object):
         config = _train_config(train_kwargs)
         solver._apply_options()
         solver._check(self._lib.gvx_session_open(self._handle, C.byref(config), int(bool(resident_pools))), "session")
-        self.open = True
+        self.open = solver._session_open = True
         solver._refresh()
         self.steps = self._lib.gvx_session_steps(self._handle)
 
@@ -167,7 +167,7 @@ class TrainingSession(object):
 
     def close(self):
         if self.open:
-            self.open = False
+            self.open = self.solver._session_open = False
             self.solver.exchange_stats = self.solver._exchange_stats()
             self.solver._check(self._lib.gvx_session_close(self._handle), "session.close")
             self.solver._refresh()
@@ -234,6 +234,7 @@ class GraphSolver(object):
                                                        int(num_sampler_per_worker), int(gpu_memory_limit))
         else:
             ids = (C.c_int * max(len(device_ids), 1))(*device_ids)
+            device = device_ids[0] if device_ids else 0
             handle = lib.gvx_solver_create(dim, ids, len(device_ids), int(num_sampler_per_worker), int(gpu_memory_limit))
         if not handle:
             message = lib.gvk_last_error().decode("utf-8", "replace")
@@ -241,6 +242,8 @@ class GraphSolver(object):
                 raise RuntimeError(message + " (graphvite_amd has no CPU training path)")
             raise ValueError(message)
         self._handle = handle
+        self.device = device  # this process's first GPU
+        self._session_open = False
         self.seed = int(seed)
         self.device_sampling = bool(device_sampling)
         self._pair_order_request = pair_order
@@ -369,6 +372,7 @@ class GraphSolver(object):
         if optimizer.type == "Default":  # what build() resolved `auto` to (solver.h:290-296; graph.cuh:634-636)
             lr = optimizer.init_lr if optimizer.init_lr > 0 else 0.025
             optimizer = SGD(lr, 5e-3, "linear")
+        self._session_open = False
         self.graph, self.optimizer = graph, optimizer
         self.num_vertex, self.num_edge = graph.num_vertex, graph.num_edge
         self.num_moment = optimizer.num_moment
@@ -440,6 +444,10 @@ class GraphSolver(object):
             raise RuntimeError("The model must be built on a graph first")
         return TrainingSession(self, resident_pools=resident_pools, **train_kwargs)
 
+    def _no_session(self, what):
+        if self._session_open:
+            raise ValueError("%s: a training session is open; close it first (its tables are written back then)" % what)
+
     # ------------------------------------------------------------------------------------------------ predict
     def predict(self, samples):
         """
@@ -459,6 +467,42 @@ class GraphSolver(object):
         self._check(self._lib.gvx_solver_predict(self._handle, pairs.ctypes.data, len(pairs), logits.ctypes.data),
                     "GraphSolver.predict")
         return logits
+
+    # ------------------------------------------------------------------------------------------------ whole rows
+    def scorer(self, device=None):
+        """
+        scorer(device=None)
+        The embeddings as they are now, ready to answer for whole rows of candidates: a LinkScorer (logits of a node against
+        every node, the best of them) with the context table in 8 bits on one GPU.
+
+        Parameters:
+            device (int, optional): GPU id, default is the solver's first
+        """
+        from .scorer import LinkScorer
+        return LinkScorer(self, device)
+
+    def distill(self, teacher, heads=None, num_epoch=1, batch_size=auto, k=64, temperature=1.0, lr=0.025, seed=None):
+        """
+        distill(teacher, heads=None, num_epoch=1, batch_size=auto, k=64, temperature=1.0, lr=0.025, seed=None)
+        Train the embeddings to answer as another model does: for every node h, softmax(<vertex[h], context> / temperature) over all
+        nodes is moved towards the teacher's, of which its k largest logits (and the sum of its whole row) are used.
+        Plain SGD on the sum of the rows' Kullback-Leibler divergences; moment tables are left alone.
+
+        Parameters:
+            teacher (LinkScorer): scorer of another solver (any dimension) over the same nodes
+            heads (ndarray, optional): ids of the nodes to learn for, each once, default is all
+            num_epoch (int): passes over the nodes
+            batch_size (int, optional): nodes per update, default is 1024, or fewer where their logits would fill more than a GiB
+            k (int): entries of the teacher's list per node, up to 256
+            temperature (float): of both softmaxes
+            lr (float): learning rate
+            seed (int, optional): of the order of the nodes, default is the solver's
+
+        Returns:
+            list of float: mean divergence per node, of every epoch
+        """
+        from .scorer import distill
+        return distill(self, teacher, heads, num_epoch, batch_size, k, temperature, lr, seed)
 
     def save_embeddings(self, file_name):
         """Save vertex embeddings in word2vec binary format: "N dim\\n", then per node its name, a space, dim raw

@@ -435,8 +435,7 @@ int gvk_describe_train(int dim, int optimizer_type, int num_negative, int explic
 
 /* ---- whole rows: logits of every candidate, the best of them, learning from them ------------------------------------------
  * gvk_predict answers for given pairs; these answer for a node against every candidate.  No counterpart in the reference's
- * node-embedding path (its knowledge-graph application ranks all entities by predicting every pair,
- * python/graphvite/application/application.py:759-847).
+ * node-embedding path.
  *
  * Element types of rows, queries, logits and gradients. */
 enum { GVK_F32 = 0, GVK_BF16 = 1, GVK_F16 = 2 };
