@@ -250,6 +250,25 @@ struct table_view {
 // twice.  So the two loads of a tile and block take whole lines, eight rows each: lane (r, g) of L0 holds row r % 8, sixteen bytes at
 // 16 g (r < 8) or 64 + 16 g (r >= 8), of L1 the same of row 8 + r % 8; halves of sixteen lanes change places (a DPP move) to make the
 // operands of it.  4096 x 65536 x d512, bf16: 388 -> 338 us together with the order of the workgroups, 1 x 1M x d512: 115 -> 102 us.
+//
+// A strip of 256 may end before its last waves begin, and a wave's 64 rows may end inside: both read the table's last row instead, and
+// nothing of what they compute from it is stored.
+constexpr __host__ __device__ uint32_t first_in_table(uint32_t first, uint32_t num_row) { return first < num_row ? first : num_row - 1; }
+constexpr __host__ __device__ uint32_t row_of_wave(uint32_t row, uint32_t first, uint32_t num_row) {
+    return row < num_row - 1 - first ? row : num_row - 1 - first;
+}
+constexpr bool strips_stay_inside(uint32_t num_row) {
+    for (uint32_t wave = 0; wave < 256; wave += 64) {
+        const uint32_t first = first_in_table((num_row - 1) / 256 * 256 + wave, num_row);
+        for (uint32_t row = 0; row < 64; row++)
+            if (first >= num_row || row_of_wave(row, first, num_row) >= num_row - first) return false;
+    }
+    return true;
+}
+static_assert(strips_stay_inside(1) && strips_stay_inside(64) && strips_stay_inside(65) && strips_stay_inside(256) && strips_stay_inside(257) &&
+                  strips_stay_inside(448) && strips_stay_inside(449) && strips_stay_inside(0x7fffff00u),
+              "a wave reads rows of the table only");
+
 struct table_rows {
     const uint8_t *values, *exponents;  // of the strip's first row: the same for the wave
     uint32_t at[4][2], exponent[4];
@@ -258,14 +277,13 @@ struct table_rows {
     __device__ __forceinline__ table_rows(const table_view &t, uint32_t first) : padded(t.padded) {
         const int lane = threadIdx.x & 63;
         column = (lane >> 4) * 16 + (lane & 8) * 8;
-        first = __builtin_amdgcn_readfirstlane(first);
+        first = __builtin_amdgcn_readfirstlane(first_in_table(first, t.num_row));
         values = t.values + (int64_t)first * t.value_stride, exponents = t.exponents + (size_t)first * t.blocks;
-        const uint32_t last = t.num_row - 1 - first;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            at[i][0] = min(i * 16u + (lane & 7), last) * (uint32_t)t.value_stride;
-            at[i][1] = min(i * 16u + 8 + (lane & 7), last) * (uint32_t)t.value_stride;
-            exponent[i] = min(i * 16u + (lane & 15), last) * t.blocks;
+            at[i][0] = row_of_wave(i * 16u + (lane & 7), first, t.num_row) * (uint32_t)t.value_stride;
+            at[i][1] = row_of_wave(i * 16u + 8 + (lane & 7), first, t.num_row) * (uint32_t)t.value_stride;
+            exponent[i] = row_of_wave(i * 16u + (lane & 15), first, t.num_row) * t.blocks;
         }
     }
     // L0 or L1 of tile i

@@ -132,6 +132,22 @@ def test_logits_against_the_oracle(hip, query_kind, kind, m, n, dim):
     assert torch.equal(again, logits)
 
 
+@pytest.mark.parametrize("n", [1, 64, 65, 192, 193, 255, 257, 320, 321, 448, 449])
+def test_strips_that_end_before_their_waves(hip, n):
+    """Tables whose last strip of 256 candidates leaves whole waves without any."""
+    rng = np.random.default_rng(n)
+    _, rows = strided(rng.standard_normal((n, 260)), "f32")
+    _, query = strided(rng.standard_normal((21, 260)), "bf16")
+    table = hip.quantize_blocks(rows)
+    out_base, out = strided(np.zeros((21, n)), "f32", 1, 2)
+    hip.block_logits(query, table, out)
+    q, x = numbers(query), table_numbers(hip, table)
+    bound = 2 * 260 * 2.0 ** -24 * (np.abs(q) @ np.abs(x).T)
+    exact = q @ x.T
+    assert (np.abs(numbers(out) - exact) <= bound + rounding("f32", exact)).all()
+    assert gaps_intact(out_base, out)
+
+
 def test_few_and_many_queries_agree(hip):
     """The two kernels add in the same order: a query's logits do not depend on how many ask with it."""
     rng = np.random.default_rng(0)
