@@ -71,6 +71,7 @@ struct top_shared {
     uint32_t count;  // of packed keys, beyond what fits, so that it is known
     uint32_t bound[WAVES];
     float reduce[WAVES], sum[WAVES];
+    uint32_t full[WAVES];
 };
 
 // Lanes with a key of a wave append it.
@@ -265,14 +266,14 @@ __global__ void __launch_bounds__(kTopThreads) top_kernel(const T *logits, int64
     }
     const bool full = __any(mine > kSlots);
     sum = wave_sum(sum);
-    if ((threadIdx.x & 63) == 0) s.sum[wave] = full ? __builtin_nanf("") : sum, s.reduce[wave] = sum;
+    if ((threadIdx.x & 63) == 0) s.sum[wave] = sum, s.full[wave] = full;  // not s.reduce: a slower wave may still read its maxima there
     __syncthreads();
-    float check = s.sum[0];
-    sum = s.reduce[0];
+    sum = s.sum[0];
+    uint32_t crowded = s.full[0];
 #pragma unroll
-    for (int w = 1; w < kTopWaves; w++) sum += s.reduce[w], check += s.sum[w];
+    for (int w = 1; w < kTopWaves; w++) sum += s.sum[w], crowded |= s.full[w];
     uint32_t count = s.count;
-    if (count > kPacked || check != check || tau == -kInfinity) {
+    if (count > kPacked || crowded || sum != sum || tau == -kInfinity) {
         const int64_t begin = max((int64_t)0, z.first(chunk0)), end = min(num_col, z.first(chunk1));
         count = collect_exactly(s, (uint32_t)min((int64_t)k, max((int64_t)0, end - begin)), [&](auto visit) {
 #pragma unroll 1
