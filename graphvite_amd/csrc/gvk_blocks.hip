@@ -16,6 +16,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "gvk.h"
 #include "gvk_internal.h"
 #include "gvk_rows.hpp"
@@ -157,9 +159,32 @@ __global__ void __launch_bounds__(256) fragment_kernel(const T *query, int64_t q
     put_fragment(fragments + ((size_t)block * tiles + row / 16) * 4 * kFragment, row % 16, c, x);
 }
 
+// the lane, made where it is asked for: neither it nor what is made of it is kept in registers all along
+__device__ __forceinline__ int lane_here() {
+    int lane = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0));
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
+
 // until this wave's global loads have arrived, those into LDS among them (s_waitcnt vmcnt(0))
 __device__ __forceinline__ void wait_for_loads() {
     __builtin_amdgcn_s_waitcnt(0x0f70);
+    asm volatile("" ::: "memory");
+}
+
+// the same for all but the last COUNT loads and stores (vmcnt(COUNT), its two high bits apart)
+template<int COUNT>
+__device__ __forceinline__ void wait_for_loads_before() {
+    static_assert(COUNT > 0 && COUNT < 64);
+    __builtin_amdgcn_s_waitcnt(0x0f70 | (COUNT & 15) | COUNT >> 4 << 14);
+    asm volatile("" ::: "memory");
+}
+
+// __syncthreads() but for what is on its way from or to memory: this wave's use of LDS is over (lgkmcnt(0)), then everyone's
+__device__ __forceinline__ void meet() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
 
@@ -192,7 +217,7 @@ template<bool WHOLE, class T>
 __device__ __forceinline__ void store_turned(wave_turn<T> &turn, T *logits, int64_t logit_stride, uint32_t m0, uint32_t num_query, uint32_t n0, uint32_t num_row,
                                              const f32x4 acc[4]) {
     constexpr int E = 16 / (int)sizeof(T), lanes = 64 / E, rows = 64 / lanes;  // lanes to a row's 64 candidates, rows to an instruction
-    const int lane = threadIdx.x & 63;
+    const int lane = lane_here();
     char *const bytes = reinterpret_cast<char *>(turn.bytes);
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -244,8 +269,8 @@ struct table_view {
 };
 
 // A wave's 64 rows of a table, four tiles of sixteen, as it walks along the columns.  Rows behind the last one are the last one (read, never
-// stored); columns behind a row's end are zero, by a mask after a load that stays inside the row: no branch, so that the
-// compiler counts the loads that are under way.
+// stored); for columns behind a row's end the block's last sixteen are read, and the queries' fragments are zero there: no branch and no mask, so
+// that nothing waits for a load before it is used.
 // The matrix operand of a tile is 16 rows x 64 bytes; read as that, a load touches 16 cache lines by half and asks the L2 for each
 // twice.  So the two loads of a tile and block take whole lines, eight rows each: lane (r, g) of L0 holds row r % 8, sixteen bytes at
 // 16 g (r < 8) or 64 + 16 g (r >= 8), of L1 the same of row 8 + r % 8; halves of sixteen lanes change places (a DPP move) to make the
@@ -275,8 +300,11 @@ struct table_rows {
     int padded, column;
 
     __device__ __forceinline__ table_rows(const table_view &t, uint32_t first) : padded(t.padded) {
+        column = ((threadIdx.x & 63) >> 4) * 16 + (threadIdx.x & 8) * 8;
+        move(t, first);
+    }
+    __device__ __forceinline__ void move(const table_view &t, uint32_t first) {
         const int lane = threadIdx.x & 63;
-        column = (lane >> 4) * 16 + (lane & 8) * 8;
         first = __builtin_amdgcn_readfirstlane(first_in_table(first, t.num_row));
         values = t.values + (int64_t)first * t.value_stride, exponents = t.exponents + (size_t)first * t.blocks;
 #pragma unroll
@@ -289,11 +317,38 @@ struct table_rows {
     // L0 or L1 of tile i
     __device__ __forceinline__ uint4 load(int i, int block, int half) const {
         const int c = block * kBlockColumns + column;
-        const uint4 raw = *reinterpret_cast<const uint4 *>(values + (at[i][half] + (uint32_t)min(c, padded - 16)));
-        const uint32_t mask = (uint32_t)((c - padded) >> 31);
-        return uint4{raw.x & mask, raw.y & mask, raw.z & mask, raw.w & mask};
+        return *reinterpret_cast<const uint4 *>(values + (at[i][half] + (uint32_t)min(c, padded - 16)));
     }
-    __device__ __forceinline__ float scale(int i, int block) const { return __uint_as_float((uint32_t)exponents[exponent[i] + block] << 23); }
+    __device__ __forceinline__ uint32_t exponent_byte(int i, int block) const { return exponents[exponent[i] + block]; }
+    struct place {};
+    __device__ __forceinline__ place at_block(int) const { return {}; }
+    __device__ __forceinline__ uint4 load(place, int i, int block, int half) const { return load(i, block, half); }
+    __device__ __forceinline__ uint32_t exponent_byte(place, int i, int block) const { return exponent_byte(i, block); }
+    __device__ __forceinline__ float scale(int i, int block) const { return __uint_as_float(exponent_byte(i, block) << 23); }
+};
+
+// The same where all 64 rows are there: the wave's own address and one offset of the lane's serve them all.
+struct whole_rows {
+    const uint8_t *values, *exponents;
+    int64_t stride;
+    int blocks, padded;
+
+    __device__ __forceinline__ whole_rows(const table_view &t, uint32_t first) : stride(t.value_stride), blocks(t.blocks), padded(t.padded) { move(t, first); }
+    __device__ __forceinline__ void move(const table_view &t, uint32_t first) {
+        first = __builtin_amdgcn_readfirstlane(first);
+        values = t.values + (int64_t)first * stride, exponents = t.exponents + (size_t)first * blocks;
+    }
+    struct place {
+        uint32_t value, exponent;
+    };
+    __device__ __forceinline__ place at_block(int block) const {
+        const int lane = lane_here();
+        return {(uint32_t)((lane & 7) * (int)stride + min(block * kBlockColumns + (lane >> 4) * 16 + (lane & 8) * 8, padded - 16)), (uint32_t)((lane & 15) * blocks)};
+    }
+    __device__ __forceinline__ uint4 load(const place &p, int i, int, int half) const {
+        return *reinterpret_cast<const uint4 *>(values + (i * 16 + half * 8) * stride + p.value);
+    }
+    __device__ __forceinline__ uint32_t exponent_byte(const place &p, int i, int block) const { return (exponents + (size_t)(i * 16) * blocks + block)[p.exponent]; }
 };
 
 template<int BANKS>
@@ -432,46 +487,70 @@ __global__ void __launch_bounds__(256, 4) narrow_kernel(const __bf16 *fragments,
 }
 
 // more columns: a workgroup makes 256 candidates x 16 * TILES queries, 64 candidates to a wave, the queries' fragments of a block of columns
-// in LDS, those of the next block and its table rows on their way meanwhile.  The workgroups that share candidates are consecutive
-// on one XCD (its L2 then serves the table's rows).
-template<int TILES, class T>
-__global__ void __launch_bounds__(256, 2) logits_kernel(const __bf16 *fragments, uint32_t tiles, uint32_t num_query, table_view table, T *logits,
-                                                        int64_t logit_stride) {
+// in LDS, those of the next block and its table rows on their way meanwhile: asked for at the block's start, the scheduler kept from
+// moving them behind the matrix instructions, and first touched when the block is over.  Workgroups stay and take one such square after
+// the other: while the last block of one is multiplied the first of the next is on its way, and the logits are stored behind those loads.
+// 4096 x 65536 x d512 bf16 328 us (838 TFLOP/s; the library's bf16 product of that shape 325), f32 343; a launch per square, with loads
+// where the scheduler put them: 372 and 387.  Of the 328 the 16 squares' four blocks take 200 (d2048: 933 us, 1179 TFLOP/s); the rest is
+// the stores, which a CU's other workgroup overlaps with its own products in part (without stores: 256).
+// Odd numbers of blocks change the buffers' roles from square to square, which takes a build with two squares to a turn.
+template<int TILES>
+constexpr int staying_groups() {  // to a CU: what registers and LDS allow
+    return TILES <= 2 ? 3 : 2;
+}
+
+template<int TILES, class T, bool WHOLE, bool ODD>
+__global__ void __launch_bounds__(256, staying_groups<TILES>()) logits_kernel(const __bf16 *fragments, uint32_t tiles, uint32_t num_query, table_view table,
+                                                                              T *logits, int64_t logit_stride) {
     // two objects, not one array: the compiler then knows that reading one does not wait for what is on its way into the other
-    constexpr int kTurns = 4 * (int)sizeof(wave_turn<T>) / 16;
-    __shared__ uint4 even[TILES * 256 > kTurns ? TILES * 256 : kTurns], odd[TILES * 256];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr int kTurns = 4 * (int)sizeof(wave_turn<T>) / 16, kStaged = TILES * 256 > kTurns ? TILES * 256 : kTurns;
+    __shared__ uint4 even[kStaged], odd[kStaged];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // An XCD's workgroups take squares of up to 8 parts x 8 strips in turn, the strips first: its L2 holds what the 64 of them read.
     const uint32_t parts = (tiles + TILES - 1) / TILES, strips = ((table.num_row + 255) / 256 + 7) / 8;  // strips of an XCD
-    const uint32_t xcd = blockIdx.x % 8, turn = blockIdx.x / 8;
-    const uint32_t side = min(parts, 8u), column = turn / (side * strips), width = min(side, parts - column * side);
-    const uint32_t inside = turn - column * side * strips, row_group = inside / (width * 8), height = min(8u, strips - row_group * 8);
-    const uint32_t rest = inside - row_group * width * 8;
-    const uint32_t part = column * side + rest / height, strip = xcd * strips + row_group * 8 + rest % height;
-    if ((uint64_t)strip * 256 >= table.num_row) return;  // the whole workgroup
-    const uint32_t first = strip * 256 + wave * 64, tile0 = part * TILES;
-    f32x4 acc[TILES][4] = {};
-    const table_rows rows(table, first);
+    const uint32_t xcd = blockIdx.x % 8, side = min(parts, 8u);
+    uint32_t turn = blockIdx.x / 8, strip = 0, tile0 = 0;
+    const auto find = [&] {  // the square of this turn or of the next that has one
+        for (; turn < parts * strips; turn += gridDim.x / 8) {
+            const uint32_t column = turn / (side * strips), width = min(side, parts - column * side);
+            const uint32_t inside = turn - column * side * strips, row_group = inside / (width * 8), height = min(8u, strips - row_group * 8);
+            const uint32_t rest = inside - row_group * width * 8;
+            strip = xcd * strips + row_group * 8 + rest % height, tile0 = (column * side + rest / height) * TILES;
+            if ((uint64_t)strip * 256 < table.num_row) return true;
+        }
+        return false;
+    };
+    if (!find()) return;  // the whole workgroup
+    // the wave's first candidate; of a table of 64 or more the last wave's are moved back to end with it
+    const auto begin = [&] { return WHOLE ? min(strip * 256 + wave * 64, table.num_row - 64) : strip * 256 + wave * 64; };
+    std::conditional_t<WHOLE, whole_rows, table_rows> rows(table, begin());
     uint4 raw[4][2];
-    float scale[4];
+    uint32_t exponent[4];
     const auto stage = [&](uint4 *into, int block) {
+        const uint32_t at = lane_here() * 8;
 #pragma unroll
         for (int i = 0; i < TILES; i++) {
             const uint32_t tile = min(tile0 + i, tiles - 1);  // tiles behind the last one: computed, never stored
-            const __bf16 *from = fragments + ((size_t)block * tiles + tile) * 4 * kFragment + threadIdx.x * 8;
+            const __bf16 *from = fragments + ((size_t)block * tiles + tile) * 4 * kFragment + wave * kFragment + at;
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
                                              (__attribute__((address_space(3))) void *)&into[i * 256 + wave * 64], 16, 0, 0);
         }
     };
-    const auto step = [&](const uint4 *staged, uint4 *other, int block) {
-        // this wave's loads into LDS have landed, then everyone's: this block is there, and the one before is done with
-        wait_for_loads();
-        __syncthreads();
-        if (block + 1 < table.blocks) stage(other, block + 1);
-        const int after = min(block + 1, table.blocks - 1);
-        float next_scale[4];
+    bool more = true;
+    const auto step = [&](const uint4 *staged, uint4 *other, int block, f32x4 (&acc)[TILES][4]) {
+        meet();  // this wave's loads into LDS had landed, and now everyone's: this block is there, and the one before is done with
+        const bool last = block + 1 == table.blocks;
+        if (last) {
+            turn += gridDim.x / 8;
+            more = find();
+            rows.move(table, begin());  // where there is no more: the same again, loaded for nothing
+        }
+        const int after = last ? 0 : block + 1;
+        if (more) stage(other, after);
+        uint32_t next_exponent[4];
+        const auto place = rows.at_block(after);
         // a fragment is asked for RING fragments before it is used: LDS answers meanwhile
-        constexpr int RING = 4;
+        constexpr int RING = 2;
         bf16x8 ring[RING];
         const auto fragment = [&](int t) {  // t = (step, tile)
             return __builtin_bit_cast(bf16x8, staged[((t % TILES) * 4 + t / TILES) * 64 + lane]);
@@ -484,13 +563,14 @@ __global__ void __launch_bounds__(256, 2) logits_kernel(const __bf16 *fragments,
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 if (j == 0) change_places(raw[i][0], raw[i][1]);
-                widen(raw[i][j], scale[i], a[i]);
+                widen(raw[i][j], __uint_as_float(exponent[i] << 23), a[i]);
             }
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                raw[i][j] = rows.load(i, after, j);
-                if (j == 0) next_scale[i] = rows.scale(i, after);
+                raw[i][j] = rows.load(place, i, after, j);
+                if (j == 0) next_exponent[i] = rows.exponent_byte(place, i, after);
             }
+            __builtin_amdgcn_sched_barrier(0);  // left alone, they are asked for at the block's end and waited for at once
 #pragma unroll
             for (int t = 2 * j * TILES; t < 2 * (j + 1) * TILES; t++) {
 #pragma unroll
@@ -501,20 +581,49 @@ __global__ void __launch_bounds__(256, 2) logits_kernel(const __bf16 *fragments,
             }
         }
 #pragma unroll
-        for (int i = 0; i < 4; i++) scale[i] = next_scale[i];
+        for (int i = 0; i < 4; i++) exponent[i] = next_exponent[i];
+        if (!last) wait_for_loads();
+    };
+    const auto square = [&](uint4 *staged, uint4 *other) {
+        const uint32_t first = begin(), first_tile = tile0;
+        const bool empty = strip * 256 + wave * 64 >= table.num_row;
+        f32x4 acc[TILES][4] = {};
+        for (int block = 0; block + 1 < table.blocks; block += 2) step(staged, other, block, acc), step(other, staged, block + 1, acc);
+        if constexpr (ODD) step(staged, other, table.blocks - 1, acc);
+        meet();                             // the turns lie over the fragments that everyone is done with
+        __builtin_amdgcn_sched_barrier(0);  // no load moves behind the stores
+        wave_turn<T> &turned = reinterpret_cast<wave_turn<T> *>(ODD ? staged : other)[wave];
+        const auto store = [&](int tile) {
+            const uint32_t m0 = (first_tile + tile) * 16;
+            store_turned<WHOLE>(turned, logits, logit_stride, WHOLE ? min(m0, num_query - 16) : m0, num_query, first, table.num_row, acc[tile]);
+        };
+        // The next square's first loads are older than these stores, and loads and stores come back in order: all but the stores having
+        // come back means that the loads have, and the stores go on.
+        if (WHOLE && !empty && first_tile + TILES <= tiles) {
+#pragma unroll
+            for (int tile = 0; tile < TILES; tile++) store(tile);
+            wait_for_loads_before<TILES * (int)sizeof(T)>();  // a wave's stores of a tile: 16 x 64 logits, sixteen bytes a lane
+        } else {
+            if (!empty) {
+#pragma unroll
+                for (int tile = 0; tile < TILES; tile++)
+                    if (first_tile + tile < tiles) store(tile);
+            }
+            wait_for_loads();
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        return more;
     };
     stage(even, 0);
+    const auto place = rows.at_block(0);
 #pragma unroll
-    for (int i = 0; i < 4; i++) raw[i][0] = rows.load(i, 0, 0), raw[i][1] = rows.load(i, 0, 1), scale[i] = rows.scale(i, 0);
-    for (int block = 0; block < table.blocks; block += 2) {
-        step(even, odd, block);
-        if (block + 1 < table.blocks) step(odd, even, block + 1);
+    for (int i = 0; i < 4; i++) raw[i][0] = rows.load(place, i, 0, 0), raw[i][1] = rows.load(place, i, 0, 1), exponent[i] = rows.exponent_byte(place, i, 0);
+    wait_for_loads();
+    if constexpr (ODD) {
+        while (square(even, odd) && square(odd, even)) {}
+    } else {
+        while (square(even, odd)) {}
     }
-    __syncthreads();  // the turns lie over the fragments
-    wave_turn<T> &turned = reinterpret_cast<wave_turn<T> *>(even)[wave];
-#pragma unroll
-    for (int tile = 0; tile < TILES; tile++)
-        store_turned<false>(turned, logits, logit_stride, (tile0 + tile) * 16, num_query, first, table.num_row, acc[tile]);
 }
 
 bool aligned(const void *p, int64_t stride_bytes, size_t to) { return (uintptr_t)p % to == 0 && stride_bytes % (int64_t)to == 0; }
@@ -557,9 +666,9 @@ int launch_logits(hipStream_t stream, const Q *query, int64_t query_stride, uint
     }
     const uint32_t tiles = (num_query + 15) / 16;
     __bf16 *fragments = reinterpret_cast<__bf16 *>(workspace);
-    const bool narrow = table.blocks == 1 && num_query > 16 && table.num_row >= 256;
+    const bool whole = num_query > 16 && table.num_row >= 64, narrow = whole && table.blocks == 1 && table.num_row >= 256;
     hipLaunchKernelGGL((fragment_kernel<Q>), dim3((tiles * 16 * table.blocks + 7) / 8), dim3(256), 0, stream, query, query_stride, query_wide,
-                       num_query, tiles, dim, table.blocks, narrow, fragments);
+                       num_query, tiles, dim, table.blocks, whole, fragments);
     const uint64_t strips = ((uint64_t)table.num_row + 255) / 256;
     if (narrow) {
         // The chip holds 1024 workgroups: as many parts as make the longest row of them on one place shortest, the table's rows counting as
@@ -575,17 +684,20 @@ int launch_logits(hipStream_t stream, const Q *query, int64_t query_stride, uint
         hipLaunchKernelGGL((narrow_kernel<T>), dim3((unsigned)grid), dim3(256), 0, stream, fragments, tiles, num_query, parts, table, logits, logit_stride);
         return launched("gvk_block_logits");
     }
-#define GVK_LOGITS(TILES)                                                                                                                 \
-    {                                                                                                                                     \
-        const uint64_t grid = (strips + 7) / 8 * 8 * ((tiles + TILES - 1) / TILES);                                                       \
-        if (grid > 0xffffffull) return gvk_fail(GVK_EINVAL, "gvk_block_logits: too many logits for one call");                          \
-        hipLaunchKernelGGL((logits_kernel<TILES, T>), dim3((unsigned)grid), dim3(256), 0, stream, fragments, tiles, num_query, table, logits, \
-                           logit_stride);                                                                                           \
+#define GVK_LOGITS(TILES, WHOLE)                                                                                                            \
+    {                                                                                                                                       \
+        const uint64_t squares = (strips + 7) / 8 * 8 * ((tiles + TILES - 1) / TILES), chip = 256 * staying_groups<TILES>();               \
+        if (squares > 0xffffffffull) return gvk_fail(GVK_EINVAL, "gvk_block_logits: too many logits for one call");                       \
+        const dim3 grid((unsigned)(squares < chip ? squares : chip));                                                                      \
+        if (table.blocks % 2)                                                                                                               \
+            hipLaunchKernelGGL((logits_kernel<TILES, T, WHOLE, true>), grid, dim3(256), 0, stream, fragments, tiles, num_query, table, logits, logit_stride); \
+        else                                                                                                                                \
+            hipLaunchKernelGGL((logits_kernel<TILES, T, WHOLE, false>), grid, dim3(256), 0, stream, fragments, tiles, num_query, table, logits, logit_stride); \
     }
-    if (tiles <= 1) GVK_LOGITS(1)
-    else if (tiles <= 2) GVK_LOGITS(2)
-    else if (tiles <= 4) GVK_LOGITS(4)
-    else GVK_LOGITS(8)
+    if (!whole) GVK_LOGITS(1, false)
+    else if (tiles <= 2) GVK_LOGITS(2, true)
+    else if (tiles <= 4) GVK_LOGITS(4, true)
+    else GVK_LOGITS(8, true)
 #undef GVK_LOGITS
     return launched("gvk_block_logits");
 }
