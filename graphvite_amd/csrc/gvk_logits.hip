@@ -31,13 +31,13 @@ __device__ __forceinline__ float reference_of(float largest) { return largest ==
 // collected in, the answer is the same.  A slice of a row (16384 logits) lives in the registers of a workgroup.  Every thread takes
 // the largest of its elements (of each quarter of them for k above 128); of a wave's 64 (256) such maxima the ceil(k / waves)-th
 // largest, and of those the least, is a bound that at least k elements reach, and only a few more than k do (normal logits,
-// k = 64: about 85).  Every lane puts those of its own into its own slots in LDS; then they are packed.  One slice: they are ranked by
+// k = 64: about 85).  Every lane marks those of its own, a bit each; those are packed.  One slice: they are ranked by
 // counting.  More: they go to a list, and one workgroup per row does the same with the lists.  Rows that defeat the bound (all logits equal,
 // NaN) take the exact way: a bisection of the key, bit by bit.
 
 constexpr int kTopThreads = 256, kTopWaves = kTopThreads / 64, kMergeThreads = 512, kMergeWaves = kMergeThreads / 64;
 constexpr uint32_t kPacked = 1024;  // keys a workgroup packs
-constexpr int kSlots = 8;           // slots of a lane
+constexpr uint32_t kKept = 4;       // chunks of a thread kept in LDS; more are read again from memory
 
 __device__ __forceinline__ uint32_t ordered(float x) {
     if (x != x) return 0xffffffffu;  // NaN above everything: it shows
@@ -48,6 +48,8 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 __device__ __forceinline__ float of_ordered(uint32_t key) { return __uint_as_float(key ^ ((key >> 31) ? 0x80000000u : 0xffffffffu)); }
 
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t index) { return (uint64_t)ordered(x) << 32 | (uint32_t)~index; }
+
+__device__ __forceinline__ float uniform(float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); }
 
 // the rank-th largest (1-based) of the 64 * N values a wave holds, its lowest 16 bits cut off: a bound that `rank` of them reach (0: not
 // that many do)
@@ -71,7 +73,6 @@ struct top_shared {
     uint32_t count;  // of packed keys, beyond what fits, so that it is known
     uint32_t bound[WAVES];
     float reduce[WAVES], sum[WAVES];
-    uint32_t full[WAVES];
 };
 
 // Lanes with a key of a wave append it.
@@ -196,7 +197,7 @@ __global__ void __launch_bounds__(kTopThreads) top_kernel(const T *logits, int64
                                                           uint32_t capacity, float scale, top_output out) {
     constexpr int E = per_chunk<T>::value;
     __shared__ top_shared<kTopWaves> s;
-    __shared__ uint64_t slots[kSlots][kTopThreads];
+    __shared__ uint4 kept[kKept][kTopThreads];
     const int64_t row = first_row + blockIdx.x / slices;
     const uint32_t slice = blockIdx.x % slices, wave = threadIdx.x >> 6;
     const chunked_row<T> z(logits + row * stride, num_col);
@@ -208,9 +209,7 @@ __global__ void __launch_bounds__(kTopThreads) top_kernel(const T *logits, int64
         return z.load(chunk < chunk1 ? chunk : chunks);  // the one behind the last reads as minus infinity
     };
     uint4 raw[U];
-#pragma unroll
-    for (int u = 0; u < U; u++) raw[u] = load(u);
-
+    z.template load<U, kTopThreads>(raw, chunk0, chunk1);
     float part[N];
     representatives<T>(raw, part);
     float largest = part[0];
@@ -237,43 +236,59 @@ __global__ void __launch_bounds__(kTopThreads) top_kernel(const T *logits, int64
         }
         m = block_max<kTopThreads>(largest, s.reduce);
     }
-    // cut bits may make a NaN of minus infinity's key
-    const float tau = least <= 0x007fffffu ? -kInfinity : of_ordered(least);
-    const float base = reference_of(m);
+    // A hair below the bound, so that what reaches it lies above, 0 and -0 alike.  Without a bound (cut bits may make a NaN of minus
+    // infinity's key) the exact way follows.
+    const bool bounded = least > 0x0080ffffu;
+    const float below = uniform(of_ordered((bounded ? least : 0x80000000u) - 16)), base = uniform(reference_of(m));
     float sum = 0;
-    // What reaches the bound is put down as it is, with its place in the slice (what lies outside the row is minus infinity and does not
-    // reach a bound above that); the keys are made of it afterwards.
-    uint32_t mine = 0;
+    // What reaches the bound: a bit per element, and the chunk it is in goes to LDS (registers take no index), a few of a thread's.  What lies outside the row is minus infinity and does not; a NaN, and infinity less
+    // infinity, are NaN in the sum too and take the exact way.
+    constexpr int kWords = (U * E + 31) / 32, kBits = U * E < 32 ? U * E : 32;
+    uint32_t hits[kWords] = {}, chunk_hits = 0, chunk_place = threadIdx.x;
 #pragma unroll
     for (int u = 0; u < U; u++) {
         float x[E];
         // 16-bit logits are unpacked again, rather than kept unpacked: 78 registers, not 152 (1024 x 1M bf16: 577 us against 631)
         if constexpr (sizeof(T) == 2) asm volatile("" : "+v"(raw[u].x), "+v"(raw[u].y), "+v"(raw[u].z), "+v"(raw[u].w), "+v"(sum));
+        else asm volatile("" : "+v"(sum), "+v"(hits[0]), "+v"(hits[kWords - 1]));
         unpack<T>(raw[u], x);
 #pragma unroll
         for (int i = 0; i < E; i++) {
             sum += exp2_fast((x[i] - base) * scale);
-            if (x[i] >= tau) {
-                slots[min(mine, (uint32_t)kSlots - 1)][threadIdx.x] = (uint64_t)__float_as_uint(x[i]) << 32 | (uint32_t)((u * kTopThreads + threadIdx.x) * E + i);
-                mine++;
-            }
+            uint32_t &word = hits[(u * E + i) / 32];
+            word = __builtin_amdgcn_alignbit(word, __float_as_uint(below - x[i]), 31);  // the sign's bit, from below
+        }
+        if (hits[u * E / 32] & ((1u << E) - 1)) {
+            if (u < (int)kKept || chunk_place < kKept * kTopThreads) (&kept[0][0])[chunk_place] = raw[u];
+            chunk_place += kTopThreads, chunk_hits |= 1u << u;
         }
     }
-    const uint32_t origin = (uint32_t)z.first(chunk0);
-    for (uint32_t slot = 0; __any(slot < mine) && slot < kSlots; slot++) {
-        const uint64_t it = slots[slot][threadIdx.x];
-        append(s, slot < mine, key_of(__uint_as_float((uint32_t)(it >> 32)), origin + (uint32_t)it));
+    // Where the elements stand in LDS and in the slice is packed: one addition to the workgroup's count for a wave.
+    uint32_t mine = 0;
+#pragma unroll
+    for (int w = 0; w < kWords; w++) mine += __popc(hits[w]);
+    uint32_t place = wave_scan(mine);
+    uint32_t before = 0;
+    if ((threadIdx.x & 63) == 63) before = atomicAdd(&s.count, place);
+    place += (uint32_t)__builtin_amdgcn_readlane((int)before, 63) - mine;
+#pragma unroll
+    for (int w = 0; w < kWords; w++) {
+        while (hits[w]) {
+            const uint32_t first = __clz(hits[w]), e = w * 32 + first - (32 - kBits), u = e / E;
+            hits[w] &= ~(0x80000000u >> first);
+            const uint32_t slot = __popc(chunk_hits & ((1u << u) - 1));
+            if (place < kPacked) s.packed[place] = (uint64_t)(slot < kKept ? ((slot * kTopThreads + threadIdx.x) * E + e % E) : ~0u) << 32 | ((u * kTopThreads + threadIdx.x) * E + e % E);
+            place++;
+        }
     }
-    const bool full = __any(mine > kSlots);
     sum = wave_sum(sum);
-    if ((threadIdx.x & 63) == 0) s.sum[wave] = sum, s.full[wave] = full;  // not s.reduce: a slower wave may still read its maxima there
+    if ((threadIdx.x & 63) == 0) s.sum[wave] = sum;  // not s.reduce: a slower wave may still read its maxima there
     __syncthreads();
     sum = s.sum[0];
-    uint32_t crowded = s.full[0];
 #pragma unroll
-    for (int w = 1; w < kTopWaves; w++) sum += s.sum[w], crowded |= s.full[w];
+    for (int w = 1; w < kTopWaves; w++) sum += s.sum[w];
     uint32_t count = s.count;
-    if (count > kPacked || crowded || sum != sum || tau == -kInfinity) {
+    if (count > kPacked || sum != sum || !bounded) {
         const int64_t begin = max((int64_t)0, z.first(chunk0)), end = min(num_col, z.first(chunk1));
         count = collect_exactly(s, (uint32_t)min((int64_t)k, max((int64_t)0, end - begin)), [&](auto visit) {
 #pragma unroll 1
@@ -285,6 +300,13 @@ __global__ void __launch_bounds__(kTopThreads) top_kernel(const T *logits, int64
                 for (int i = 0; i < E; i++) visit(at + i >= 0 && at + i < end, key_of(x[i], (uint32_t)(at + i)));
             }
         });
+    } else {
+        const T *const elements = reinterpret_cast<const T *>(kept);
+        for (uint32_t i = threadIdx.x; i < count; i += kTopThreads) {
+            const uint64_t it = s.packed[i];
+            const uint32_t at = (uint32_t)z.first(chunk0) + (uint32_t)it, from = (uint32_t)(it >> 32);
+            s.packed[i] = key_of(to_float(from == ~0u ? z.row[at] : elements[from]), at);
+        }
     }
     if (slices == 1) {
         write_ranked(s, count, k, [&](uint32_t rank, uint64_t key) {
@@ -545,8 +567,7 @@ __global__ void __launch_bounds__(THREADS) distill_row_kernel(distill_input in, 
     const int64_t row = first_row + blockIdx.x;
     const chunked_row<T> z((const T *)in.logits + row * in.stride, in.num_col);
     uint4 raw[U];
-#pragma unroll
-    for (int u = 0; u < U; u++) raw[u] = z.load(u * THREADS + threadIdx.x);
+    z.template load<U, THREADS>(raw, 0, z.chunks());
     if constexpr (GRAD)
         for (int i = threadIdx.x; i < SIZE / 32 + 1; i += THREADS) l.bits[i] = 0;
     const row_answer r = solve_row<THREADS>(
@@ -622,8 +643,7 @@ __global__ void __launch_bounds__(kSliceThreads) distill_partial_kernel(distill_
     const uint32_t slice = blockIdx.x % slices;
     const chunked_row<T> z((const T *)in.logits + row * in.stride, in.num_col);
     uint4 raw[U];
-#pragma unroll
-    for (int u = 0; u < U; u++) raw[u] = z.load((int64_t)(slice * (uint64_t)U + u) * kSliceThreads + threadIdx.x);
+    z.template load<U, kSliceThreads>(raw, (int64_t)slice * (U * kSliceThreads), z.chunks());
     float largest = -kInfinity;
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -705,8 +725,7 @@ __global__ void __launch_bounds__(kSliceThreads) distill_grad_kernel(distill_inp
     const chunked_row<T> z((const T *)in.logits + row * in.stride, in.num_col);
     const int64_t chunk0 = (int64_t)slice * (U * kSliceThreads), begin = z.first(chunk0);
     uint4 raw[U];
-#pragma unroll
-    for (int u = 0; u < U; u++) raw[u] = z.load(chunk0 + u * kSliceThreads + threadIdx.x);
+    z.template load<U, kSliceThreads>(raw, chunk0, z.chunks());
     const float4 f = out.factors[local];
     for (int i = threadIdx.x; i < kSliceElements / 32 + 1; i += kSliceThreads) l.bits[i] = 0;
     __syncthreads();
