@@ -31,10 +31,12 @@ __device__ __forceinline__ float reference_of(float largest) { return largest ==
 // collected in, the answer is the same.  A slice of a row (16384 logits) lives in the registers of a workgroup.  Every thread takes
 // the largest of its elements (of each quarter of them for k above 128); of a wave's 64 (256) such maxima the ceil(k / waves)-th
 // largest, and of those the least, is a bound that at least k elements reach, and only a few more than k do (normal logits,
-// k = 64: about 85).  Every lane marks those of its own, a bit each; those are packed.  One slice: they are ranked by
-// counting.  More: they go to a list, and one workgroup per row does the same with the lists.  Rows that defeat the bound (all logits equal,
-// NaN) take the exact way: a bisection of the key, bit by bit.
-
+// k = 64: about 85).  Every lane marks those of its own, a bit each, and puts the chunks they are in into LDS; then they are packed, one
+// addition to the count for a wave.  One slice: they are ranked by counting.  More: they go to a list, and one workgroup per row does the
+// same with the lists.  Rows that defeat the bound (all logits equal, NaN) take the exact way: a bisection of the key, bit by bit.
+// Seven instructions an element, the exponential at a quarter of the rate: 512 x 1M f32 378 us (5.4 TB/s, what reading a row's slices
+// reaches), 1024 x 1M bf16 500 (4.1 TB/s: twice the elements a byte, both count), of those 25 the lists; without collecting at all 350
+// and 400.  Collecting elements one by one as they are met, 450 and 565: four instructions each, and an atomic a round.
 constexpr int kTopThreads = 256, kTopWaves = kTopThreads / 64, kMergeThreads = 512, kMergeWaves = kMergeThreads / 64;
 constexpr uint32_t kPacked = 1024;  // keys a workgroup packs
 constexpr uint32_t kKept = 4;       // chunks of a thread kept in LDS; more are read again from memory
@@ -327,8 +329,13 @@ __global__ void __launch_bounds__(kTopThreads) top_kernel(const T *logits, int64
     if (threadIdx.x == 0) out.counts[list] = count, out.partial[list] = make_float2(m, sum);
 }
 
-// The lists of a row's slices -> its top entries and statistics.  A wave takes every eighth list, several at a time; the bound is the k-th
-// largest of all threads' largest keys (waves have lists of different lengths, or none).
+// The lists of a row's slices -> its top entries and statistics.  CACHED: sixteen keys to a thread hold all the lists, which are read once;
+// the lists' 64-entry pieces are dealt to the waves in turn, from another wave on every time (a list's last pieces are emptier than its
+// first).  Else a wave takes every eighth list, several at a time, and reads them twice.  The bound is the k-th largest of all threads'
+// largest keys.
+constexpr int kCached = 16;
+
+template<bool CACHED>
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(int64_t first_row, uint32_t slices, uint32_t k, uint32_t log_capacity, float scale, top_output out) {
     __shared__ top_shared<kMergeWaves> s;
     __shared__ uint32_t maxima[kMergeThreads];
@@ -336,8 +343,24 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(int64_t first_row,
     const uint64_t list0 = (uint64_t)blockIdx.x * slices;
     const uint64_t *const keys = out.lists + (list0 << log_capacity);
     const uint32_t *const counts = out.counts + list0;
-    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63, slots = slices << log_capacity;
+    uint64_t cached[kCached] = {};  // no key is 0
+    if constexpr (CACHED) {
+        uint32_t length[kCached];
+        const auto slot = [&](uint32_t r) { return r * kMergeThreads + ((wave + r) % kMergeWaves) * 64 + lane; };
+#pragma unroll
+        for (int r = 0; r < kCached; r++) length[r] = slot(r) < slots ? counts[slot(r) >> log_capacity] : 0;
+#pragma unroll
+        for (int r = 0; r < kCached; r++)
+            if ((slot(r) & ((1u << log_capacity) - 1)) < length[r]) cached[r] = keys[slot(r)];
+    }
     const auto each = [&](auto visit) {
+        if constexpr (CACHED) {
+#pragma unroll
+            for (int r = 0; r < kCached; r++)
+                if (r * kMergeThreads < slots) visit(cached[r] != 0, cached[r]);
+            return;
+        }
         constexpr int kTogether = 4;
         for (uint32_t l = wave; l < slices; l += kMergeWaves * kTogether) {
             uint32_t count[kTogether], longest = 0;
@@ -356,17 +379,18 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(int64_t first_row,
         }
     };
     if (threadIdx.x == 0) s.count = 0;
+    const float2 part = threadIdx.x < slices ? out.partial[list0 + threadIdx.x] : make_float2(-kInfinity, 0.0f);
     uint32_t largest = 0;
     each([&](bool valid, uint64_t key) {
         if (valid) largest = max(largest, (uint32_t)(key >> 32));
     });
     maxima[threadIdx.x] = largest;
-    float m = -kInfinity, sum = 0;
-    for (uint32_t i = threadIdx.x; i < slices; i += kMergeThreads) m = fmaxf(m, out.partial[list0 + i].x);
+    float m = part.x, sum = 0;
+    for (uint32_t i = threadIdx.x + kMergeThreads; i < slices; i += kMergeThreads) m = fmaxf(m, out.partial[list0 + i].x);
     m = block_max<kMergeThreads>(m, s.reduce);  // its barriers publish the maxima too
     const float base = reference_of(m);
     for (uint32_t i = threadIdx.x; i < slices; i += kMergeThreads) {
-        const float2 p = out.partial[list0 + i];
+        const float2 p = i == threadIdx.x ? part : out.partial[list0 + i];
         if (p.x > -kInfinity || p.y != p.y) sum += p.y * exp2_fast((reference_of(p.x) - base) * scale);  // not a slice of nothing but masks
     }
     uint32_t all[kMergeWaves];
@@ -810,8 +834,12 @@ void launch_top(hipStream_t stream, const top_plan &p, const T *logits, int64_t 
     else if (k <= 128) GVK_TOP(kSmall, 1);
     else GVK_TOP(kSmall, 4);
 #undef GVK_TOP
-    if (p.slices > 1)
-        hipLaunchKernelGGL(merge_kernel, dim3((unsigned)num_row), dim3(kMergeThreads), 0, stream, first_row, (uint32_t)p.slices, (uint32_t)k, (uint32_t)p.log_capacity, scale, out);
+    if (p.slices > 1) {
+        const bool cached = (p.slices << p.log_capacity) <= kCached * kMergeThreads;
+        const dim3 rows((unsigned)num_row);
+        if (cached) hipLaunchKernelGGL((merge_kernel<true>), rows, dim3(kMergeThreads), 0, stream, first_row, (uint32_t)p.slices, (uint32_t)k, (uint32_t)p.log_capacity, scale, out);
+        else hipLaunchKernelGGL((merge_kernel<false>), rows, dim3(kMergeThreads), 0, stream, first_row, (uint32_t)p.slices, (uint32_t)k, (uint32_t)p.log_capacity, scale, out);
+    }
 }
 
 constexpr int64_t kRowElements = 16384;  // a row that a workgroup of 1024 threads holds
