@@ -131,7 +131,7 @@ class ApplicationMixin(object):
 
     @_timed
     def evaluate(self, task, **kwargs):
-        """evaluate(task, **kwargs): evaluate the learned embeddings on a downstream task; returns a dict."""
+        """evaluate(task, **kwargs): evaluate the learned embeddings on a downstream task; returns a dict (neighbor prediction: a list)."""
         func_name = task.replace(" ", "_")
         if not hasattr(self, func_name):
             raise ValueError("Unknown task `%s`" % task)
@@ -331,7 +331,7 @@ class GraphApplication(ApplicationMixin):
     def neighbor_prediction(self, H=None, file_name=None, k=10):
         """
         Predict the k most likely neighbors of each node: the nodes with the largest score = <vertex[h], context[t]> of all, scored with
-        the context table in 8 bits (GraphSolver.scorer).  The node-embedding counterpart of the reference's entity prediction.
+        the context table in 8 bits (GraphSolver.scorer).
 
         Parameters:
             H (list, optional): nodes
@@ -346,7 +346,10 @@ class GraphApplication(ApplicationMixin):
         ids = self.get_mapping([str(h) for h in H], self.graph.name2id)
         index, scores, _ = self.solver.scorer().top(ids, k)
         id2name = self.graph.id2name
-        return [[(id2name[int(t)], float(score)) for t, score in zip(*row)] for row in zip(index, scores)]
+        answers = [[(id2name[int(t)], float(score)) for t, score in zip(*row)] for row in zip(index, scores)]
+        for h, answer in zip(H, answers):
+            logger.info("%s: %s", h, ", ".join("%s (%g)" % pair for pair in answer))
+        return answers
 
 
 def linear_classification(embeddings, labels, portion, normalization=False, times=1, patience=100):

@@ -1,6 +1,6 @@
 """Thin, typed Python face of the kernel ABI (include/gvk.h) over torch tensors.
 
-torch supplies device memory and streams only; every computation is a libgvk.so kernel.
+torch supplies device memory and streams only; every computation here is a libgvk.so kernel (`scorer.distill` adds two plain torch products).
 A `HipKernels` object is what `solver.GraphSolver` calls; tests for the host logic may inject an object
 (the CPU tests run the engine over tests/hostdev instead: the same entry points served by the CPU oracle).
 """
