@@ -44,19 +44,21 @@ __device__ __forceinline__ uint32_t exponent_of(uint32_t largest) {
 
 __device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// the largest of a half wave (32 lanes: one block of columns, four to a lane)
+// the largest of a half wave (32 lanes: one block of columns, four to a lane), of numbers below 2^31
 __device__ __forceinline__ uint32_t half_wave_max(uint32_t v) {
-#pragma unroll
-    for (int step = 1; step < 32; step <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, step));
-    return v;
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xb1, 0xf, 0xf, true));   // quad_perm [1 0 3 2]
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4e, 0xf, 0xf, true));   // quad_perm [2 3 0 1]
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, true));  // row_half_mirror
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, true));  // row_mirror
+    return max(v, (uint32_t)__shfl_xor((int)v, 16));
 }
 
 // four e4m3 bytes of x * 2^(127 - exponent), rounded to nearest even; NaN bytes where the block is marked
 __device__ __forceinline__ uint32_t quantise4(const float x[4], uint32_t exponent) {
-    if (exponent == 255) return 0x7f7f7f7fu;
     const int shift = 127 - (int)exponent;
     int packed = __builtin_amdgcn_cvt_pk_fp8_f32(ldexpf(x[0], shift), ldexpf(x[1], shift), 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(ldexpf(x[2], shift), ldexpf(x[3], shift), packed, true);
+    packed = __builtin_amdgcn_cvt_pk_fp8_f32(ldexpf(x[2], shift), ldexpf(x[3], shift), packed, true);
+    return exponent == 255 ? 0x7f7f7f7fu : (uint32_t)packed;
 }
 
 // columns [column, column + 4) of a row as floats, zero behind its end
@@ -433,30 +435,45 @@ struct group_turn {
     uint4 bytes[2][16 * pitch / 16];
 };
 
-template<class T>
-__global__ void __launch_bounds__(256, 4) narrow_kernel(const __bf16 *fragments, uint32_t tiles, uint32_t num_query, uint32_t parts, table_view table, T *logits,
-                                                        int64_t logit_stride) {
+// ALONE: no launch before this one; a part is one or two tiles, and every workgroup lays out its own.
+template<bool ALONE, class Q, class T>
+__global__ void __launch_bounds__(256, ALONE ? 3 : 4) narrow_kernel(const Q *query, int64_t query_stride, bool query_wide, int dim, const __bf16 *fragments, uint32_t tiles,
+                                                                    uint32_t num_query, uint32_t parts, table_view table, T *logits, int64_t logit_stride) {
     __shared__ group_turn<T> turns;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ __bf16 own[ALONE ? 2 * 4 * kFragment : 8];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t xcd = blockIdx.x % 8, turn = blockIdx.x / 8;
     const uint32_t part = turn % parts, strip = xcd * (gridDim.x / 8 / parts) + turn / parts;
     if ((uint64_t)strip * 256 >= table.num_row) return;
     const uint32_t first = min(strip * 256, table.num_row - 256);
-    const table_rows rows(table, first + wave * 64);
+    const uint32_t begin = (uint32_t)((uint64_t)tiles * part / parts), end = (uint32_t)((uint64_t)tiles * (part + 1) / parts);
+    const whole_rows rows(table, first + wave * 64);
+    const auto place = rows.at_block(0);
+    uint4 raw[4][2];
+    uint32_t exponent[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) raw[i][0] = rows.load(place, i, 0, 0), raw[i][1] = rows.load(place, i, 0, 1), exponent[i] = rows.exponent_byte(place, i, 0);
+    if constexpr (ALONE) {
+        for (uint32_t item = threadIdx.x / 32; item < (end - begin) * 16; item += 8) {  // a half wave takes a row, four columns to a lane
+            const uint32_t tile = begin + item / 16, c = (threadIdx.x & 31) * 4;
+            float x[4];
+            load4(query + (int64_t)(min(tile * 16, num_query - 16) + item % 16) * query_stride, (int)c, dim, query_wide, x);
+            put_fragment(own + item / 16 * 4 * kFragment, item % 16, c, x);
+        }
+        __syncthreads();
+    }
     bf16x8 a[4][4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const float scale = rows.scale(i, 0);
-        uint4 l0 = rows.load(i, 0, 0), l1 = rows.load(i, 0, 1);
-        change_places(l0, l1);
-        widen(l0, scale, a[i]), widen(l1, scale, a[i] + 2);
+        const float scale = __uint_as_float(exponent[i] << 23);
+        change_places(raw[i][0], raw[i][1]);
+        widen(raw[i][0], scale, a[i]), widen(raw[i][1], scale, a[i] + 2);
     }
-    const uint32_t begin = (uint32_t)((uint64_t)tiles * part / parts), end = (uint32_t)((uint64_t)tiles * (part + 1) / parts);
-    const bf16x8 *const at = reinterpret_cast<const bf16x8 *>(fragments) + lane;
     bf16x8 b[4];
     const auto fetch = [&](uint32_t tile) {
+        const bf16x8 *const at = reinterpret_cast<const bf16x8 *>(ALONE ? own : fragments) + (size_t)(ALONE ? tile - begin : tile) * 4 * 64 + lane;
 #pragma unroll
-        for (int s = 0; s < 4; s++) b[s] = at[(size_t)(tile * 4 + s) * 64];
+        for (int s = 0; s < 4; s++) b[s] = at[s * 64];
     };
     constexpr int E = 16 / (int)sizeof(T), lanes = 256 / E, rows_at_once = 64 / lanes;  // lanes to a row, rows to an instruction of a wave
     fetch(begin);
@@ -667,8 +684,10 @@ int launch_logits(hipStream_t stream, const Q *query, int64_t query_stride, uint
     const uint32_t tiles = (num_query + 15) / 16;
     __bf16 *fragments = reinterpret_cast<__bf16 *>(workspace);
     const bool whole = num_query > 16 && table.num_row >= 64, narrow = whole && table.blocks == 1 && table.num_row >= 256;
-    hipLaunchKernelGGL((fragment_kernel<Q>), dim3((tiles * 16 * table.blocks + 7) / 8), dim3(256), 0, stream, query, query_stride, query_wide,
-                       num_query, tiles, dim, table.blocks, whole, fragments);
+    const auto lay_out = [&] {
+        hipLaunchKernelGGL((fragment_kernel<Q>), dim3((tiles * 16 * table.blocks + 7) / 8), dim3(256), 0, stream, query, query_stride, query_wide,
+                           num_query, tiles, dim, table.blocks, whole, fragments);
+    };
     const uint64_t strips = ((uint64_t)table.num_row + 255) / 256;
     if (narrow) {
         // The chip holds 1024 workgroups: as many parts as make the longest row of them on one place shortest, the table's rows counting as
@@ -681,9 +700,19 @@ int launch_logits(hipStream_t stream, const Q *query, int64_t query_stride, uint
         }
         const uint64_t grid = (strips + 7) / 8 * 8 * parts;
         if (grid > 0xffffffull) return gvk_fail(GVK_EINVAL, "gvk_block_logits: too many logits for one call");
-        hipLaunchKernelGGL((narrow_kernel<T>), dim3((unsigned)grid), dim3(256), 0, stream, fragments, tiles, num_query, parts, table, logits, logit_stride);
+        // Few tiles to a workgroup (50 x 10312: one): laying them out where they are used takes 1 us a tile, a launch before this one 2.5
+        // (7.5 us against 10; at eight tiles, 256 x 100000, 22 against 19).
+        if ((tiles + parts - 1) / parts <= 2) {
+            hipLaunchKernelGGL((narrow_kernel<true, Q, T>), dim3((unsigned)grid), dim3(256), 0, stream, query, query_stride, query_wide, dim, nullptr, tiles, num_query, parts,
+                               table, logits, logit_stride);
+            return launched("gvk_block_logits");
+        }
+        lay_out();
+        hipLaunchKernelGGL((narrow_kernel<false, __bf16, T>), dim3((unsigned)grid), dim3(256), 0, stream, nullptr, 0, false, dim, fragments, tiles, num_query, parts, table, logits,
+                           logit_stride);
         return launched("gvk_block_logits");
     }
+    lay_out();
 #define GVK_LOGITS(TILES, WHOLE)                                                                                                            \
     {                                                                                                                                       \
         const uint64_t squares = (strips + 7) / 8 * 8 * ((tiles + TILES - 1) / TILES), chip = 256 * staying_groups<TILES>();               \
