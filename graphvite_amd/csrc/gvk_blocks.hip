@@ -569,8 +569,9 @@ __global__ void __launch_bounds__(256, staying_groups<TILES>()) logits_kernel(co
         // a fragment is asked for RING fragments before it is used: LDS answers meanwhile
         constexpr int RING = 2;
         bf16x8 ring[RING];
+        const uint4 *const mine = staged + lane_here();
         const auto fragment = [&](int t) {  // t = (step, tile)
-            return __builtin_bit_cast(bf16x8, staged[((t % TILES) * 4 + t / TILES) * 64 + lane]);
+            return __builtin_bit_cast(bf16x8, mine[((t % TILES) * 4 + t / TILES) * 64]);
         };
 #pragma unroll
         for (int t = 0; t < RING && t < 4 * TILES; t++) ring[t] = fragment(t);
