@@ -302,6 +302,17 @@ __global__ void __launch_bounds__(kTopThreads) top_kernel(const T *logits, int64
                 for (int i = 0; i < E; i++) visit(at + i >= 0 && at + i < end, key_of(x[i], (uint32_t)(at + i)));
             }
         });
+        if constexpr (!representative_is_largest<T>()) {  // a NaN among a thread's elements hides their largest
+            float largest = -kInfinity;
+#pragma unroll 1
+            for (int u = 0; u < U; u++) {
+                float x[E];
+                unpack<T>(load(u), x);
+#pragma unroll
+                for (int i = 0; i < E; i++) largest = fmaxf(largest, x[i]);
+            }
+            m = block_max<kTopThreads>(largest, s.reduce);
+        }
     } else {
         const T *const elements = reinterpret_cast<const T *>(kept);
         for (uint32_t i = threadIdx.x; i < count; i += kTopThreads) {

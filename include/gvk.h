@@ -470,7 +470,7 @@ int gvk_block_logits(void *stream, int query_dtype, const void *query, int64_t n
 
 /* The k largest logits of each row, largest first, of equal ones the lowest candidate: values[r][0 .. k) (as floats, exactly; -0 as 0),
  * index[r][0 .. k).  NaN counts as the largest.  Minus infinity is a logit like others (a masked candidate; it comes last).
- * stats[r] = {m, log sum_j exp((z_j - m) / temperature)}, m = max_j z_j, or null; {-inf, -inf} where every logit is minus infinity, NaN in the
+ * stats[r] = {m, log sum_j exp((z_j - m) / temperature)}, m = max_j z_j (NaN aside), or null; {-inf, -inf} where every logit is minus infinity, NaN in the
  * second place where a logit is NaN or plus infinity.  1 <= k <= min(num_col, GVK_MAX_TOP).  Workspace as above. */
 size_t gvk_top_logits_workspace(int dtype, int64_t num_row, int64_t num_col, int k);
 int gvk_top_logits(void *stream, int dtype, const void *logits, int64_t num_row, int64_t num_col, int64_t stride, int k, float temperature, float *values,

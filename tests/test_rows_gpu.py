@@ -279,6 +279,67 @@ def test_top_logits_shows_nan_and_infinity(hip):
         assert np.isinf(numbers(stats)[2:, 0]).all()
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n", [40, 3000, 70000])
+def test_top_logits_with_nan_beside_the_largest(hip, kind, n):
+    """A NaN of either sign next to the row's largest logit: the NaN comes first, the largest after it, and m is the largest all the same."""
+    z = np.random.default_rng(n).standard_normal((4, n)) - 10.0
+    for r, (nan, large) in enumerate([(np.nan, 3.0), (-np.nan, 3.0), (np.nan, -2.0), (-np.nan, -2.0)]):
+        z[r, n // 2], z[r, n // 2 + 1] = nan, large
+    view = strided(z, kind)[1]
+    values, index, stats = torch.empty(4, 3, device=DEV), torch.empty(4, 3, dtype=torch.int32, device=DEV), torch.empty(4, 2, device=DEV)
+    hip.top_logits(view, values, index, stats)
+    want_values, want_index, want_stats = rows_oracle.top(numbers(view), 3, 1.0)
+    np.testing.assert_array_equal(index.cpu().numpy(), want_index)
+    np.testing.assert_array_equal(numbers(values), want_values)
+    np.testing.assert_array_equal(numbers(stats)[:, 0], want_stats[:, 0])
+    assert np.isnan(numbers(stats)[:, 1]).all()
+
+
+def test_calls_from_two_threads_on_two_streams(hip):
+    """Two host threads, a stream each, the same calls over inputs of their own, interleaved as they come: every answer is what one thread gets."""
+    import threading
+
+    def inputs(seed):
+        g = torch.Generator(device=DEV)
+        g.manual_seed(seed)
+        return torch.randn(40, 200, generator=g, device=DEV), torch.randn(30011, 200, generator=g, device=DEV)
+
+    def answers(query, rows):
+        table = hip.quantize_blocks(rows)
+        logits = torch.empty(40, 30011, device=DEV)
+        hip.block_logits(query, table, logits)
+        values, index = torch.empty(40, 50, device=DEV), torch.empty(40, 50, dtype=torch.int32, device=DEV)
+        stats, loss, grad = torch.empty(40, 2, device=DEV), torch.empty(40, device=DEV), torch.empty_like(logits)
+        hip.top_logits(logits, values, index, stats)
+        hip.distill(logits, index, values + 1, loss, stats, grad=grad)
+        return logits, values, index, loss, grad
+
+    given = [inputs(1), inputs(2)]
+    want = [answers(*x) for x in given]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(which):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(15):
+                    got = answers(*given[which])
+                    stream.synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, want[which])):
+                        wrong.append(which)
+        except Exception as e:  # shown by the main thread
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(which,)) for which in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 def test_rows_behind_the_32_bit_line(hip):
     """Row starts beyond 2^32 elements: 5 rows 2^30 apart."""
     stride, n = 1 << 30, 3000
