@@ -340,13 +340,11 @@ __global__ void __launch_bounds__(kTopThreads) top_kernel(const T *logits, int64
     if (threadIdx.x == 0) out.counts[list] = count, out.partial[list] = make_float2(m, sum);
 }
 
-// The lists of a row's slices -> its top entries and statistics.  CACHED: sixteen keys to a thread hold all the lists, which are read once;
+// The lists of a row's slices -> its top entries and statistics.  CACHED keys to a thread hold all the lists, which are read once;
 // the lists' 64-entry pieces are dealt to the waves in turn, from another wave on every time (a list's last pieces are emptier than its
-// first).  Else a wave takes every eighth list, several at a time, and reads them twice.  The bound is the k-th largest of all threads'
+// first).  CACHED 0: a wave takes every eighth list, several at a time, and reads them twice.  The bound is the k-th largest of all threads'
 // largest keys.
-constexpr int kCached = 16;
-
-template<bool CACHED>
+template<int CACHED>
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(int64_t first_row, uint32_t slices, uint32_t k, uint32_t log_capacity, float scale, top_output out) {
     __shared__ top_shared<kMergeWaves> s;
     __shared__ uint32_t maxima[kMergeThreads];
@@ -355,20 +353,20 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(int64_t first_row,
     const uint64_t *const keys = out.lists + (list0 << log_capacity);
     const uint32_t *const counts = out.counts + list0;
     const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63, slots = slices << log_capacity;
-    uint64_t cached[kCached] = {};  // no key is 0
-    if constexpr (CACHED) {
-        uint32_t length[kCached];
+    uint64_t cached[CACHED ? CACHED : 1] = {};  // no key is 0
+    if constexpr (CACHED > 0) {
+        uint32_t length[CACHED];
         const auto slot = [&](uint32_t r) { return r * kMergeThreads + ((wave + r) % kMergeWaves) * 64 + lane; };
 #pragma unroll
-        for (int r = 0; r < kCached; r++) length[r] = slot(r) < slots ? counts[slot(r) >> log_capacity] : 0;
+        for (int r = 0; r < CACHED; r++) length[r] = slot(r) < slots ? counts[slot(r) >> log_capacity] : 0;
 #pragma unroll
-        for (int r = 0; r < kCached; r++)
+        for (int r = 0; r < CACHED; r++)
             if ((slot(r) & ((1u << log_capacity) - 1)) < length[r]) cached[r] = keys[slot(r)];
     }
     const auto each = [&](auto visit) {
-        if constexpr (CACHED) {
+        if constexpr (CACHED > 0) {
 #pragma unroll
-            for (int r = 0; r < kCached; r++)
+            for (int r = 0; r < CACHED; r++)
                 if (r * kMergeThreads < slots) visit(cached[r] != 0, cached[r]);
             return;
         }
@@ -846,10 +844,14 @@ void launch_top(hipStream_t stream, const top_plan &p, const T *logits, int64_t 
     else GVK_TOP(kSmall, 4);
 #undef GVK_TOP
     if (p.slices > 1) {
-        const bool cached = (p.slices << p.log_capacity) <= kCached * kMergeThreads;
+        const int64_t slots = p.slices << p.log_capacity;
         const dim3 rows((unsigned)num_row);
-        if (cached) hipLaunchKernelGGL((merge_kernel<true>), rows, dim3(kMergeThreads), 0, stream, first_row, (uint32_t)p.slices, (uint32_t)k, (uint32_t)p.log_capacity, scale, out);
-        else hipLaunchKernelGGL((merge_kernel<false>), rows, dim3(kMergeThreads), 0, stream, first_row, (uint32_t)p.slices, (uint32_t)k, (uint32_t)p.log_capacity, scale, out);
+#define GVK_MERGE(CACHED) \
+    hipLaunchKernelGGL((merge_kernel<CACHED>), rows, dim3(kMergeThreads), 0, stream, first_row, (uint32_t)p.slices, (uint32_t)k, (uint32_t)p.log_capacity, scale, out)
+        if (slots <= 16 * kMergeThreads) GVK_MERGE(16);
+        else if (slots <= 32 * kMergeThreads) GVK_MERGE(32);
+        else GVK_MERGE(0);
+#undef GVK_MERGE
     }
 }
 
