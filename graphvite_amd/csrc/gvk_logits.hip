@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(kTopThreads) top_kernel(const T *logits, int64
     float sum = 0;
     // What reaches the bound: a bit per element, and the chunk it is in goes to LDS (registers take no index), a few of a thread's.  What lies outside the row is minus infinity and does not; a NaN, and infinity less
     // infinity, are NaN in the sum too and take the exact way.
-    constexpr int kWords = (U * E + 31) / 32, kBits = U * E < 32 ? U * E : 32;
+    constexpr int kWords = (U * E + 31) / 32;
     uint32_t hits[kWords] = {}, chunk_hits = 0, chunk_place = threadIdx.x;
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(kTopThreads) top_kernel(const T *logits, int64
 #pragma unroll
     for (int w = 0; w < kWords; w++) {
         while (hits[w]) {
-            const uint32_t first = __clz(hits[w]), e = w * 32 + first - (32 - kBits), u = e / E;
+            const uint32_t first = __clz(hits[w]), e = w * 32 + first - (32 - min(32, U * E - w * 32)), u = e / E;  // the word's bits end with its lowest
             hits[w] &= ~(0x80000000u >> first);
             const uint32_t slot = __popc(chunk_hits & ((1u << u) - 1));
             if (place < kPacked) s.packed[place] = (uint64_t)(slot < kKept ? ((slot * kTopThreads + threadIdx.x) * E + e % E) : ~0u) << 32 | ((u * kTopThreads + threadIdx.x) * E + e % E);
@@ -463,7 +463,7 @@ struct row_answer {
 //   largest() / sum(base)   a thread's part of max z and of S
 //   seen(i)                 whether candidate i was listed before (by an entry that got there first)
 //   logit(i)                z_i
-//   place(i, q)             called for every entry with its probability, before the last barrier
+//   place(e, i)             called for every entry and its candidate, before the last barrier
 // An index outside the row makes the row's answer NaN: it shows, and nothing is read or written out of bounds.  Nothing is to be
 // learned from a row without entries, whatever its logits hold, nor from one whose candidates are all masked: loss and gradient 0.
 template<int THREADS, class Largest, class Sum, class Seen, class Logit, class Place>
@@ -525,7 +525,7 @@ __device__ __forceinline__ row_answer solve_row(const distill_input &in, int64_t
             const float shifted = (s.q[e] - mt) / in.temperature;
             q = in.teacher_stats ? expf(shifted - lt) : expf(shifted) * inverse;
             if (!(q == 0)) loss += q * ((shifted - lt) - ((logit(i) - r.m) / in.temperature - r.log_sum));  // 0 log 0 = 0
-            place(i, q);
+            place(e, i);
         }
         s.q[e] = q;
         q_total += q;
@@ -565,12 +565,11 @@ __device__ __forceinline__ void join_repeated(uint32_t k, const list_shared<THRE
     }
 }
 
-// What the gradient of a stretch of elements takes from the list: a bit per element that has a share, and there the share, or which
-// entry of the list holds it.
-template<int SIZE, class Share>
+// What the gradient of a stretch of elements takes from the list: a bit per element that has a share, and which entry of the list holds it.
+template<int SIZE>
 struct listed_slice {
     uint32_t bits[SIZE / 32 + 1];
-    Share share[SIZE];
+    uint16_t share[SIZE];
 };
 
 // gradient of a chunk: p_factor = w Q / (T S); share(place) is subtracted where the list has one
@@ -591,12 +590,15 @@ __device__ __forceinline__ void chunk_gradient(const uint4 raw, int place, float
     }
 }
 
-// Rows that fit a workgroup's registers: read once, written once, one launch.  U chunks to a thread.
+// Rows that fit a workgroup's registers: read once, written once, one launch.  U chunks to a thread.  What bounds many rows is how many of them
+// a CU holds (they wait for their loads and three barriers each): few threads with many chunks, builds near the row's length, the
+// list's entries by their 16-bit place.  4000 x 10312 bf16, a step: 37 us; 1024 threads, 16384 elements and shares of 32 bits: 89.
+// 4000 x 16000 f32 98 (5.2 TB/s) against 134; a few rows are no slower (50 x 10312 f32: 9.5).
 template<class T, int THREADS, int U, bool GRAD>
 __global__ void __launch_bounds__(THREADS) distill_row_kernel(distill_input in, distill_output out, int64_t first_row) {
     constexpr int E = per_chunk<T>::value, SIZE = THREADS * U * E;
     __shared__ list_shared<THREADS> s;
-    __shared__ listed_slice<GRAD ? SIZE : 32, float> l;
+    __shared__ listed_slice<GRAD ? SIZE : 32> l;
     const int64_t row = first_row + blockIdx.x;
     const chunked_row<T> z((const T *)in.logits + row * in.stride, in.num_col);
     uint4 raw[U];
@@ -634,8 +636,8 @@ __global__ void __launch_bounds__(THREADS) distill_row_kernel(distill_input in, 
             return (atomicOr(&l.bits[at >> 5], bit) & bit) != 0;
         },
         [&](int32_t i) { return to_float(z.row[i]); },
-        [&](int32_t i, float q) {
-            if constexpr (GRAD) l.share[i + z.lead] = q;
+        [&](uint32_t e, int32_t i) {
+            if constexpr (GRAD) l.share[i + z.lead] = (uint16_t)e;
         });
     if (threadIdx.x == 0) {
         out.loss[row] = r.loss;
@@ -643,7 +645,8 @@ __global__ void __launch_bounds__(THREADS) distill_row_kernel(distill_input in, 
     }
     if constexpr (GRAD) {
         if (r.repeated) {
-            join_repeated(in.k, s, [&](uint32_t, int32_t i, float q) { l.share[i + z.lead] = q; });
+            // in place: of a candidate's entries only the first one's q changes, and no other thread reads that
+            join_repeated(in.k, s, [&](uint32_t e, int32_t i, float q) { s.q[e] = q, l.share[i + z.lead] = (uint16_t)e; });
             __syncthreads();
         }
         const float base = reference_of(r.m), q_factor = (in.weight ? in.weight[row] : 1.0f) / in.temperature, p_factor = q_factor * r.q_total / r.sum;
@@ -653,7 +656,7 @@ __global__ void __launch_bounds__(THREADS) distill_row_kernel(distill_input in, 
         for (int u = 0; u < U; u++) {
             const int place = (u * THREADS + (int)threadIdx.x) * E;
             float g[E];
-            chunk_gradient<T>(raw[u], place, base, in.scale, p_factor, r.nothing, l.bits, [&](int at) { return l.share[at] * q_factor; }, g);
+            chunk_gradient<T>(raw[u], place, base, in.scale, p_factor, r.nothing, l.bits, [&](int at) { return s.q[l.share[at]] * q_factor; }, g);
             store_chunk<T>(grad, (int64_t)place - z.lead, in.num_col, wide, g);
         }
     }
@@ -735,7 +738,7 @@ __global__ void __launch_bounds__(kSliceThreads) distill_finish_kernel(distill_i
                 if (was == i) return true;
             }
         },
-        [&](int32_t i) { return GIVEN ? 0.0f : to_float(z[i]); }, [](int32_t, float) {});
+        [&](int32_t i) { return GIVEN ? 0.0f : to_float(z[i]); }, [](uint32_t, int32_t) {});
     if (!GIVEN && threadIdx.x == 0) {
         out.loss[row] = r.loss;
         out.stats[2 * row] = r.m, out.stats[2 * row + 1] = r.log_sum;
@@ -752,7 +755,7 @@ __global__ void __launch_bounds__(kSliceThreads) distill_finish_kernel(distill_i
 template<class T>
 __global__ void __launch_bounds__(kSliceThreads) distill_grad_kernel(distill_input in, distill_output out, int64_t first_row, uint32_t slices) {
     constexpr int E = per_chunk<T>::value, U = slice_chunks<T>();
-    __shared__ listed_slice<kSliceElements, uint16_t> l;
+    __shared__ listed_slice<kSliceElements> l;
     const int64_t local = blockIdx.x / slices, row = first_row + local;
     const uint32_t slice = blockIdx.x % slices;
     const chunked_row<T> z((const T *)in.logits + row * in.stride, in.num_col);
@@ -810,10 +813,10 @@ int check_temperature(const char *who, float temperature, float *scale) {
 // slices a row of num_col takes wherever in 16 bytes it begins
 int64_t slices_of(int64_t num_col, int64_t slice, int per_chunk) { return (num_col + per_chunk - 1 + slice - 1) / slice; }
 
-constexpr int64_t kTopSlice = 16384, kTopSmallSlice = 4096;
+constexpr int64_t kTopSlice = 16384, kTopStep = 4096;
 
 struct top_plan {
-    int64_t slice, slices;
+    int64_t slice, slices;  // a row of one slice takes the shortest build that holds it
     int log_capacity;
     size_t bytes;
 };
@@ -821,9 +824,9 @@ struct top_plan {
 top_plan plan_top(int dtype, int64_t num_row, int64_t num_col, int k) {
     const int per_chunk = 16 / (int)size_of(dtype);
     top_plan p;
+    p.slices = slices_of(num_col, kTopSlice, per_chunk);
     p.slice = kTopSlice;
-    p.slices = slices_of(num_col, p.slice, per_chunk);
-    if (slices_of(num_col, kTopSmallSlice, per_chunk) == 1) p.slice = kTopSmallSlice, p.slices = 1;
+    while (p.slices == 1 && p.slice > kTopStep && slices_of(num_col, p.slice - kTopStep, per_chunk) == 1) p.slice -= kTopStep;
     p.log_capacity = 6;
     while ((1 << p.log_capacity) < 2 * k) p.log_capacity++;
     p.bytes = p.slices > 1 ? (size_t)num_row * p.slices * ((8ull << p.log_capacity) + sizeof(float2) + sizeof(uint32_t)) : 0;
@@ -833,15 +836,19 @@ top_plan plan_top(int dtype, int64_t num_row, int64_t num_col, int k) {
 template<class T>
 void launch_top(hipStream_t stream, const top_plan &p, const T *logits, int64_t stride, int64_t first_row, int64_t num_row, int64_t num_col, int k, float scale,
                 const top_output &out) {
-    constexpr int E = per_chunk<T>::value, kLarge = kTopSlice / kTopThreads / E, kSmall = kTopSmallSlice / kTopThreads / E;
+    constexpr int kChunks = kTopStep / kTopThreads / per_chunk<T>::value;
     const dim3 grid((unsigned)(num_row * p.slices));
-#define GVK_TOP(U, N)                                                                                                                              \
-    hipLaunchKernelGGL((top_kernel<T, U, N>), grid, dim3(kTopThreads), 0, stream, logits, stride, first_row, (uint32_t)p.slices, num_col, (uint32_t)k, \
-                       1u << p.log_capacity, scale, out)
-    if (p.slice == kTopSlice && k <= 128) GVK_TOP(kLarge, 1);
-    else if (p.slice == kTopSlice) GVK_TOP(kLarge, 4);
-    else if (k <= 128) GVK_TOP(kSmall, 1);
-    else GVK_TOP(kSmall, 4);
+#define GVK_TOP(STEPS)                                                                                                                                              \
+    if (k <= 128)                                                                                                                                                  \
+        hipLaunchKernelGGL((top_kernel<T, STEPS * kChunks, 1>), grid, dim3(kTopThreads), 0, stream, logits, stride, first_row, (uint32_t)p.slices, num_col, (uint32_t)k, \
+                           1u << p.log_capacity, scale, out);                                                                                                      \
+    else                                                                                                                                                           \
+        hipLaunchKernelGGL((top_kernel<T, STEPS * kChunks, 4>), grid, dim3(kTopThreads), 0, stream, logits, stride, first_row, (uint32_t)p.slices, num_col, (uint32_t)k, \
+                           1u << p.log_capacity, scale, out)
+    if (p.slice == kTopStep) GVK_TOP(1);
+    else if (p.slice == 2 * kTopStep) GVK_TOP(2);
+    else if (p.slice == 3 * kTopStep) GVK_TOP(3);
+    else GVK_TOP(4);
 #undef GVK_TOP
     if (p.slices > 1) {
         const int64_t slots = p.slices << p.log_capacity;
@@ -868,8 +875,11 @@ void launch_rows(hipStream_t stream, const distill_input &in, const distill_outp
 #define GVK_ROWS(THREADS, ELEMENTS) \
     hipLaunchKernelGGL((distill_row_kernel<T, THREADS, ELEMENTS / THREADS / E, GRAD>), dim3(rows), dim3(THREADS), 0, stream, in, out, first)
     if (need <= 2048) GVK_ROWS(256, 2048);
+    else if (need <= 4096) GVK_ROWS(256, 4096);
+    else if (need <= 6144) GVK_ROWS(256, 6144);
     else if (need <= 8192) GVK_ROWS(512, 8192);
-    else GVK_ROWS(1024, 16384);
+    else if (need <= 12288) GVK_ROWS(512, 12288);
+    else GVK_ROWS(512, 16384);
 #undef GVK_ROWS
 }
 

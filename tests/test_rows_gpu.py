@@ -262,6 +262,18 @@ def test_top_logits_of_rows_that_defeat_the_bound(hip, kind, n):
         check_top(hip, strided(z, kind)[1], k, 1.0)
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n", [4088, 4097, 8185, 8193, 12281, 12289, 16377, 16385])
+def test_top_logits_at_the_sizes_between_builds(hip, kind, n):
+    """Rows that just fit a build and rows that just do not, beginning on sixteen bytes and elsewhere; the last elements among the largest."""
+    z = np.random.default_rng(n).standard_normal((3, n))
+    z[:, -3:] += 5
+    z[0, :9] += 5
+    for lead, extra in ((0, 8 - n % 8), (1, 0)):
+        for k in (5, 64, 200):
+            check_top(hip, strided(z, kind, lead, extra)[1], k, 1.0)
+
+
 def test_top_logits_shows_nan_and_infinity(hip):
     for n in (50, 30000):
         z = np.random.default_rng(n).standard_normal((4, n))
@@ -463,6 +475,19 @@ def test_distill_against_the_oracle(hip, kind, rows, n, k, lead, extra):
     check_distill(hip, view, index, teacher, 1.0)
     check_distill(hip, view, index, teacher, 2.0, teacher_stats=teacher_stats, weight=weight, grad_lead=1, grad_extra=3)
     check_distill(hip, view, index, teacher, 0.5, weight=-weight if whole else None, grad_lead=lead, grad_extra=extra)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [2041, 2049, 4089, 4097, 6137, 6145, 8185, 8193, 12281, 12289, 16377, 16385])
+def test_distill_at_the_sizes_between_builds(hip, kind, n):
+    """As above, with entries on the row's first and last candidates, and one of them twice."""
+    rng = np.random.default_rng(n)
+    z = rng.standard_normal((3, n))
+    index = np.stack([rng.permutation(n)[:40] for _ in range(3)]).astype(np.int32)
+    index[:, :3] = (0, n - 1, n // 2)
+    index[1, 7] = index[1, 30] = n - 1
+    for lead, extra in ((0, 8 - n % 8), (1, 0)):
+        check_distill(hip, strided(z, kind, lead, extra)[1], index, (rng.standard_normal((3, 40)) * 2).astype(np.float32), 1.5, grad_lead=lead)
 
 
 @pytest.mark.parametrize("n", [200, 3000, 33000])
