@@ -40,6 +40,8 @@ class LinkScorer(object):
         if solver.graph is None:
             raise RuntimeError("The model must be built on a graph first")
         solver._no_session("scorer")
+        if not torch.cuda.is_available():
+            raise RuntimeError("a scorer answers on a GPU; graphvite_amd has no CPU path for it")
         self.device = torch.device("cuda", solver.device if device is None else int(device))
         self.graph, self.dim, self.num_vertex = solver.graph, solver.dim, solver.num_vertex
         self.kernels = HipKernels()

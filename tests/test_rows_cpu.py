@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import rows_oracle
-from graphvite_amd import _lib
+from graphvite_amd import _lib, scorer
 from graphvite_amd.kernels import BlockTable, HipKernels
 
 P = C.c_void_p(1 << 20)  # never followed: every call below is refused (or has nothing to do) before a launch
@@ -185,3 +185,41 @@ def test_the_oracle_against_torch():
         down[1, j] -= 1e-5
         slope = (rows_oracle.distill(up, index, t, 2.0)[0][1] - rows_oracle.distill(down, index, t, 2.0)[0][1]) / 2e-5
         assert abs(2.0 * slope - grad[1, j]) < 1e-9
+
+
+class _Built(object):
+    """What a scorer asks of a solver before it touches a GPU."""
+    graph, device, num_vertex, seed = object(), 0, 5, 0
+
+    def __init__(self, session=False):
+        self.session = session
+
+    def _no_session(self, what):
+        if self.session:
+            raise ValueError("%s: a training session is open" % what)
+
+
+def test_scorer_and_distill_refuse_before_any_gpu():
+    unbuilt = _Built()
+    unbuilt.graph = None
+    for call in (lambda s: scorer.LinkScorer(s), lambda s: scorer.distill(s, None)):
+        with pytest.raises(RuntimeError, match="must be built"):
+            call(unbuilt)
+        with pytest.raises(ValueError, match="session is open"):
+            call(_Built(session=True))
+    with pytest.raises(TypeError, match="LinkScorer"):
+        scorer.distill(_Built(), _Built())
+    if not torch.cuda.is_available():
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            scorer.LinkScorer(_Built())
+
+
+@pytest.mark.parametrize("bad", [[[1]], [0.5], [-1], [5], "1"])
+def test_node_rows_refuses(bad):
+    with pytest.raises(ValueError):
+        scorer.node_rows(bad, 5, "cpu")
+
+
+def test_node_rows():
+    assert scorer.node_rows(np.array([4, 0, 4], np.uint32), 5, "cpu").tolist() == [4, 0, 4]
+    assert scorer.node_rows(np.zeros(0, np.int64), 5, "cpu").shape == (0,)
