@@ -47,6 +47,7 @@ class LinkScorer(object):
         self.kernels = HipKernels()
         self.vertex = torch.from_numpy(solver.vertex_embeddings).to(self.device)
         self.table = self.kernels.quantize_blocks(torch.from_numpy(solver.context_embeddings).to(self.device))
+        torch.cuda.current_stream(self.device).synchronize()  # whichever stream asks first finds the table whole
 
     def logits(self, heads, dtype=torch.float32):
         """

@@ -58,6 +58,20 @@ def test_scorer_answers_from_the_8_bit_table(edges, dim):
     assert scorer.top(np.zeros(0, np.int64), 3)[0].shape == (0, 3)
 
 
+def test_scorer_made_on_one_stream_answers_on_another(edges):
+    g, s = solver_with(512, edges, 8)
+    heads = np.arange(40)
+    want = s.scorer().top(heads, 30)
+    made, asked = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(5):
+        with torch.cuda.stream(made):
+            scorer = s.scorer()
+        with torch.cuda.stream(asked):
+            got = scorer.top(heads, 30)
+        for a, b in zip(got, want):
+            np.testing.assert_array_equal(a, b)
+
+
 def test_scorer_refuses(edges):
     g, s = solver_with(32, edges, 1)
     scorer = s.scorer()
