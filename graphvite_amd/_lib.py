@@ -116,6 +116,36 @@ class NativeLibraryError(RuntimeError):
 _lib = None
 
 
+def _bind_whole_rows(l):
+    """The entry points of whole rows of candidates.  They came to include/gvk.h after the training path: a library made before them
+    loads and trains all the same, and says which of them it lacks when it is called."""
+    vp, i32, f32, size = C.c_void_p, C.c_int, C.c_float, C.c_size_t
+    wide = C.c_int64  # rows, columns and strides
+    for name, restype, argtypes in (
+            ("gvk_block_quantize", i32, [vp, i32, vp, wide, i32, wide, vp, wide, vp]),
+            ("gvk_block_dequantize", i32, [vp, vp, wide, vp, wide, i32, i32, vp, wide]),
+            ("gvk_block_logits_workspace", size, [wide, i32]),
+            ("gvk_block_logits", i32, [vp, i32, vp, wide, wide, vp, wide, vp, wide, i32, i32, vp, wide, vp, size]),
+            ("gvk_top_logits_workspace", size, [i32, wide, wide, i32]),
+            ("gvk_top_logits", i32, [vp, i32, vp, wide, wide, wide, i32, f32, vp, vp, vp, vp, size]),
+            ("gvk_distill_workspace", size, [i32, wide, wide, i32]),
+            ("gvk_distill", i32, [vp, i32, vp, wide, wide, wide, i32, vp, vp, vp, f32, vp, vp, vp, vp, wide, vp, size]),
+            ("gvk_distill_grad_workspace", size, [i32, wide, wide, i32]),
+            ("gvk_distill_grad", i32, [vp, i32, vp, wide, wide, wide, i32, vp, vp, vp, f32, vp, vp, vp, wide, vp, size])):
+        function = getattr(l, name, None)
+        if function is None:
+            setattr(l, name, _missing(name))
+        else:
+            function.restype, function.argtypes = restype, argtypes
+
+
+def _missing(name):
+    def call(*args):
+        raise NativeLibraryError("%s has no %s: it was built before whole rows of candidates (include/gvk.h), or is not the product "
+                                 "library; build it again (`make -C graphvite_amd/csrc`)" % (LIB_PATH, name))
+    return call
+
+
 def lib():
     """The loaded library. torch is imported first so that libgvk.so binds to the HIP runtime torch uses
     (streams and device pointers cross the boundary, so there must be exactly one runtime in the process)."""
@@ -158,27 +188,7 @@ def lib():
                                           i32, i32, f32, vp, C.c_size_t, u32, u32, i32, i32, i32, i32, i32, i32]
     l.gvk_predict.restype = i32
     l.gvk_predict.argtypes = [vp, i32, vp, vp, vp, vp, i32]
-    wide = C.c_int64  # rows, columns and strides
-    l.gvk_block_quantize.restype = i32
-    l.gvk_block_quantize.argtypes = [vp, i32, vp, wide, i32, wide, vp, wide, vp]
-    l.gvk_block_dequantize.restype = i32
-    l.gvk_block_dequantize.argtypes = [vp, vp, wide, vp, wide, i32, i32, vp, wide]
-    l.gvk_block_logits_workspace.restype = C.c_size_t
-    l.gvk_block_logits_workspace.argtypes = [wide, i32]
-    l.gvk_block_logits.restype = i32
-    l.gvk_block_logits.argtypes = [vp, i32, vp, wide, wide, vp, wide, vp, wide, i32, i32, vp, wide, vp, C.c_size_t]
-    l.gvk_top_logits_workspace.restype = C.c_size_t
-    l.gvk_top_logits_workspace.argtypes = [i32, wide, wide, i32]
-    l.gvk_top_logits.restype = i32
-    l.gvk_top_logits.argtypes = [vp, i32, vp, wide, wide, wide, i32, f32, vp, vp, vp, vp, C.c_size_t]
-    l.gvk_distill_workspace.restype = C.c_size_t
-    l.gvk_distill_workspace.argtypes = [i32, wide, wide, i32]
-    l.gvk_distill.restype = i32
-    l.gvk_distill.argtypes = [vp, i32, vp, wide, wide, wide, i32, vp, vp, vp, f32, vp, vp, vp, vp, wide, vp, C.c_size_t]
-    l.gvk_distill_grad_workspace.restype = C.c_size_t
-    l.gvk_distill_grad_workspace.argtypes = [i32, wide, wide, i32]
-    l.gvk_distill_grad.restype = i32
-    l.gvk_distill_grad.argtypes = [vp, i32, vp, wide, wide, wide, i32, vp, vp, vp, f32, vp, vp, vp, wide, vp, C.c_size_t]
+    _bind_whole_rows(l)
     l.gvk_probe_row_traffic.restype = i32
     l.gvk_probe_row_traffic.argtypes = [vp, i32, vp, vp, vp, vp, C.c_float, i32]
     l.gvk_alias_sample.restype = i32

@@ -445,32 +445,6 @@ int gvk_predict(void *, int dim, const float *vertex, const float *context, cons
     return GVK_OK;
 }
 
-// whole rows of candidates: device kernels only
-size_t gvk_block_logits_workspace(int64_t, int) { return 0; }
-size_t gvk_top_logits_workspace(int, int64_t, int64_t, int) { return 0; }
-size_t gvk_distill_workspace(int, int64_t, int64_t, int) { return 0; }
-size_t gvk_distill_grad_workspace(int, int64_t, int64_t, int) { return 0; }
-int gvk_block_quantize(void *, int, const void *, int64_t, int, int64_t, uint8_t *, int64_t, uint8_t *) {
-    return gvk_fail(GVK_EHIP, "gvk_block_quantize: not part of the host build");
-}
-int gvk_block_dequantize(void *, const uint8_t *, int64_t, const uint8_t *, int64_t, int, int, void *, int64_t) {
-    return gvk_fail(GVK_EHIP, "gvk_block_dequantize: not part of the host build");
-}
-int gvk_block_logits(void *, int, const void *, int64_t, int64_t, const uint8_t *, int64_t, const uint8_t *, int64_t, int, int, void *, int64_t, void *, size_t) {
-    return gvk_fail(GVK_EHIP, "gvk_block_logits: not part of the host build");
-}
-int gvk_top_logits(void *, int, const void *, int64_t, int64_t, int64_t, int, float, float *, int32_t *, float *, void *, size_t) {
-    return gvk_fail(GVK_EHIP, "gvk_top_logits: not part of the host build");
-}
-int gvk_distill(void *, int, const void *, int64_t, int64_t, int64_t, int, const int32_t *, const float *, const float *, float, const float *, float *, float *,
-                void *, int64_t, void *, size_t) {
-    return gvk_fail(GVK_EHIP, "gvk_distill: not part of the host build");
-}
-int gvk_distill_grad(void *, int, const void *, int64_t, int64_t, int64_t, int, const int32_t *, const float *, const float *, float, const float *, const float *,
-                     void *, int64_t, void *, size_t) {
-    return gvk_fail(GVK_EHIP, "gvk_distill_grad: not part of the host build");
-}
-
 int gvk_alias_sample(void *, const gvk_alias_entry *, uint32_t, const double *, uint32_t *, int) {
     return gvk_fail(GVK_EHIP, "gvk_alias_sample: not part of the host build");
 }
