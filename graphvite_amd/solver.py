@@ -115,7 +115,7 @@ class TrainingSession(object):
         config = _train_config(train_kwargs)
         solver._apply_options()
         solver._check(self._lib.gvx_session_open(self._handle, C.byref(config), int(bool(resident_pools))), "session")
-        self.open = solver._session_open = True
+        self.open = True
         solver._refresh()
         self.steps = self._lib.gvx_session_steps(self._handle)
 
@@ -167,7 +167,7 @@ class TrainingSession(object):
 
     def close(self):
         if self.open:
-            self.open = self.solver._session_open = False
+            self.open = False
             self.solver.exchange_stats = self.solver._exchange_stats()
             self.solver._check(self._lib.gvx_session_close(self._handle), "session.close")
             self.solver._refresh()
@@ -243,7 +243,6 @@ class GraphSolver(object):
             raise ValueError(message)
         self._handle = handle
         self.device = device  # this process's first GPU
-        self._session_open = False
         self.seed = int(seed)
         self.device_sampling = bool(device_sampling)
         self._pair_order_request = pair_order
@@ -372,7 +371,6 @@ class GraphSolver(object):
         if optimizer.type == "Default":  # what build() resolved `auto` to (solver.h:290-296; graph.cuh:634-636)
             lr = optimizer.init_lr if optimizer.init_lr > 0 else 0.025
             optimizer = SGD(lr, 5e-3, "linear")
-        self._session_open = False
         self.graph, self.optimizer = graph, optimizer
         self.num_vertex, self.num_edge = graph.num_vertex, graph.num_edge
         self.num_moment = optimizer.num_moment
@@ -445,7 +443,7 @@ class GraphSolver(object):
         return TrainingSession(self, resident_pools=resident_pools, **train_kwargs)
 
     def _no_session(self, what):
-        if self._session_open:
+        if self._lib.gvx_session_steps(self._handle):  # the engine's word: train(), build() and clear() end a session too
             raise ValueError("%s: a training session is open; close it first (its tables are written back then)" % what)
 
     # ------------------------------------------------------------------------------------------------ predict
