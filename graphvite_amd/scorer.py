@@ -109,6 +109,9 @@ def distill(solver, teacher, heads=None, num_epoch=1, batch_size=0, k=64, temper
     solver._no_session("distill")
     if not isinstance(teacher, LinkScorer):
         raise TypeError("teacher must be a LinkScorer (GraphSolver.scorer() of the solver to learn from)")
+    if solver.num_local_worker < solver.num_worker:  # every rank's tables are alike after train(), and would not be after this
+        raise ValueError("distill trains the tables of one process, and this solver's are shared by a job of %d; use a solver made outside of the job "
+                         "(its embeddings may be set to these)" % solver.num_worker)
     if teacher.graph is not solver.graph and list(teacher.graph.id2name) != list(solver.graph.id2name):
         raise ValueError("the teacher's nodes are not this solver's nodes")
     n = solver.num_vertex

@@ -484,7 +484,8 @@ class GraphSolver(object):
         distill(teacher, heads=None, num_epoch=1, batch_size=auto, k=64, temperature=1.0, lr=0.025, seed=None)
         Train the embeddings to answer as another model does: for every node h, softmax(<vertex[h], context> / temperature) over all
         nodes is moved towards the teacher's, of which its k largest logits (and the sum of its whole row) are used.
-        Plain SGD on the sum of the rows' Kullback-Leibler divergences; moment tables are left alone.
+        Plain SGD on the sum of the rows' Kullback-Leibler divergences; moment tables are left alone.  For a solver of one process
+        (any number of GPUs): one that shares its tables with the other processes of a job refuses.
 
         Parameters:
             teacher (LinkScorer): scorer of another solver (any dimension) over the same nodes

@@ -63,6 +63,28 @@ def sessions():
     assert not refused_for_a_session(s)
 
 
+def _rank(rank, port):
+    import torch.distributed as dist
+    from graphvite_amd.scorer import LinkScorer
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE="2", LOCAL_RANK=str(rank), LOCAL_WORLD_SIZE="2")
+    dist.init_process_group("gloo", rank=rank, world_size=2)
+    try:
+        _, s = make_solver()
+        s.train(model="LINE", num_epoch=1, augmentation_step=1, log_frequency=100000)
+        before = s.vertex_embeddings.copy(), s.context_embeddings.copy()
+        with pytest.raises(ValueError, match="job of 2"):
+            s.distill(LinkScorer.__new__(LinkScorer))
+        assert (s.vertex_embeddings == before[0]).all() and (s.context_embeddings == before[1]).all()
+    finally:
+        dist.destroy_process_group()
+
+
+def two_processes():
+    import torch.multiprocessing as mp
+    from host_scenarios import _free_port
+    mp.spawn(_rank, args=(_free_port(),), nprocs=2, join=True)
+
+
 @pytest.fixture(scope="module")
 def run(request):
     import json
@@ -84,6 +106,10 @@ def run(request):
 
 def test_a_session_s_state_is_the_engine_s(run):
     run("sessions")
+
+
+def test_distill_refuses_in_a_job_of_several_processes(run):
+    run("two_processes")
 
 
 if __name__ == "__main__":
