@@ -479,26 +479,31 @@ class GraphSolver(object):
         from .scorer import LinkScorer
         return LinkScorer(self, device)
 
-    def distill(self, teacher, heads=None, num_epoch=1, batch_size=auto, k=64, temperature=1.0, lr=0.025, seed=None):
+    def distill(self, teacher, heads=None, num_epoch=10, batch_size=auto, k=64, temperature=1.0, lr=auto, seed=None):
         """
-        distill(teacher, heads=None, num_epoch=1, batch_size=auto, k=64, temperature=1.0, lr=0.025, seed=None)
-        Train the embeddings to answer as another model does: for every node h, softmax(<vertex[h], context> / temperature) over all
-        nodes is moved towards the teacher's, of which its k largest logits (and the sum of its whole row) are used.
-        Plain SGD on the sum of the rows' Kullback-Leibler divergences; moment tables are left alone.  For a solver of one process
-        (any number of GPUs): one that shares its tables with the other processes of a job refuses.
+        distill(teacher, heads=None, num_epoch=10, batch_size=auto, k=64, temperature=1.0, lr=auto, seed=None)
+        Train the embeddings to answer as another model does: for every node h, p = softmax(<vertex[h], context> / temperature) over all
+        nodes is moved towards the teacher's best.  With q the teacher's probabilities (of its whole row) of its k largest logits and Q
+        their sum, plain SGD on the sum over the nodes of sum q (log q - log p); moment tables are left alone.  That is the listed part
+        of the Kullback-Leibler divergence: it can be negative, and is least (Q log Q) where p = q / Q on the list and 0 elsewhere.
+        Embeddings of a solver that was built and never trained (all zero) begin at random.  For a solver of one process (any number of
+        GPUs): one that shares its tables with the other processes of a job refuses.
 
         Parameters:
             teacher (LinkScorer): scorer of another solver (any dimension) over the same nodes
             heads (ndarray, optional): ids of the nodes to learn for, each once, default is all
             num_epoch (int): passes over the nodes
-            batch_size (int, optional): nodes per update, default is 1024, or fewer where their logits would fill more than a GiB
+            batch_size (int, optional): nodes per update, default is 256, or fewer where their logits would fill more than a GiB
             k (int): entries of the teacher's list per node, up to 256
             temperature (float): of both softmaxes
-            lr (float): learning rate
-            seed (int, optional): of the order of the nodes, default is the solver's
+            lr (float, optional): learning rate, default is temperature^2 / (2 Q max(1, H)), H = batch_size times the largest share of
+                all lists' probability that one node has
+            seed (int, optional): of the order of the nodes and of the start, default is the solver's
 
         Returns:
-            list of float: mean divergence per node, of every epoch
+            list of float: that sum per node, the mean of every epoch
+
+        An epoch that ends without a finite mean raises RuntimeError and leaves the embeddings as they were.
         """
         from .scorer import distill
         return distill(self, teacher, heads, num_epoch, batch_size, k, temperature, lr, seed)
