@@ -49,7 +49,16 @@ class LinkScorer(object):
         self.kernels = HipKernels()
         self.vertex = torch.from_numpy(solver.vertex_embeddings).to(self.device)
         self.table = self.kernels.quantize_blocks(torch.from_numpy(solver.context_embeddings).to(self.device))
-        torch.cuda.current_stream(self.device).synchronize()  # whichever stream asks first finds the table whole
+        self._made_on = torch.cuda.current_stream(self.device)
+        self._made_on.synchronize()  # whichever stream asks first finds the table whole
+
+    def _ask(self):
+        """The embeddings' memory belongs to the stream they were made on: where another one asks, it is not handed on before that one has
+        passed the question, also if the scorer is dropped meanwhile."""
+        stream = torch.cuda.current_stream(self.device)
+        if stream != self._made_on:
+            for t in (self.vertex, self.table.values, self.table.exponents):
+                t.record_stream(stream)
 
     def logits(self, heads, dtype=torch.float32):
         """
@@ -65,12 +74,14 @@ class LinkScorer(object):
         """
         with torch.cuda.device(self.device):
             rows = node_rows(heads, self.num_vertex, self.device)
+            self._ask()
             out = torch.empty((len(rows), self.num_vertex), dtype=dtype, device=self.device)
             return self.kernels.block_logits(self.vertex[rows], self.table, out)
 
     def top_on_device(self, rows, k, temperature=1.0):
         """(logits float32 [n, k], index int32 [n, k], stats float32 [n, 2]) of an index tensor on the scorer's GPU; HipKernels.top_logits."""
         n, device = len(rows), self.device
+        self._ask()
         values = torch.empty((n, k), dtype=torch.float32, device=device)
         index = torch.empty((n, k), dtype=torch.int32, device=device)
         stats = torch.empty((n, 2), dtype=torch.float32, device=device)
