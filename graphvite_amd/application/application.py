@@ -328,15 +328,17 @@ class GraphApplication(ApplicationMixin):
         auc = float(hit[Y == 0].sum()) / total if total else float("nan")
         return {"AUC": auc}
 
-    def neighbor_prediction(self, H=None, file_name=None, k=10):
+    def neighbor_prediction(self, H=None, file_name=None, k=10, scorer=None):
         """
-        Predict the k most likely neighbors of each node: the nodes with the largest score = <vertex[h], context[t]> of all, scored with
-        the context table in 8 bits (GraphSolver.scorer).
+        Predict the k most likely neighbors of each node: the nodes with the largest score = <vertex[h], context[t]> of all, the node itself
+        and the neighbors it has among them, scored with both sides in 8 bits (GraphSolver.scorer).
 
         Parameters:
             H (list, optional): nodes
             file_name (str, optional): file with one node per line
             k (int): up to 256
+            scorer (LinkScorer, optional): what answers, by default one that is made for this call from the embeddings as they are; a program
+                that asks often keeps one (self.solver.scorer()), and makes another when it has trained
 
         Returns:
             list of lists of (node, score), for each node the best first
@@ -344,7 +346,11 @@ class GraphApplication(ApplicationMixin):
         if self.one_source((H,), file_name, "Node"):
             (H,) = self.read_columns(file_name, 1, "node file")
         ids = self.get_mapping([str(h) for h in H], self.graph.name2id)
-        index, scores, _ = self.solver.scorer().top(ids, k)
+        if scorer is None:
+            scorer = self.solver.scorer()
+        elif scorer.graph is not self.graph:
+            raise ValueError("the scorer is of another graph")
+        index, scores, _ = scorer.top(ids, k)
         id2name = self.graph.id2name
         answers = [[(id2name[int(t)], float(score)) for t, score in zip(*row)] for row in zip(index, scores)]
         for h, answer in zip(H, answers):
