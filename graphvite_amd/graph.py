@@ -36,6 +36,11 @@ class _Id2Name(Sequence):
     def __len__(self):
         return self._g.num_vertex
 
+    def __iter__(self):
+        name, buf, size = _lib.lib().gvs_graph_id2name, C.create_string_buffer(64), 64
+        for i in range(len(self)):
+            yield buf.value.decode() if name(self._g._handle, i, buf, size) < size else self[i]
+
     def __getitem__(self, i):
         if isinstance(i, slice):
             return [self[j] for j in range(*i.indices(len(self)))]

@@ -3,7 +3,25 @@
 Chung-Lu style: both endpoints of every edge are drawn independently from a Zipf-like node distribution
 (expected degree of node i proportional to (i + 1)^(-1 / (gamma - 1))); self loops are redrawn, duplicate edges
 are kept (the reference's Graph keeps multi-edges too, include/instance/graph.cuh:124-153)."""
+import os
+from concurrent.futures import ThreadPoolExecutor
+
 import numpy as np
+
+
+def _search(ascending, values, side="left"):
+    """np.searchsorted, its values dealt over the threads this process may use (it holds no lock): 20M draws from a distribution over 1M nodes."""
+    threads = min(16, len(os.sched_getaffinity(0)), len(values) // 65536)
+    if threads < 2:
+        return np.searchsorted(ascending, values, side=side)
+    out = np.empty(len(values), np.intp)
+    cuts = np.linspace(0, len(values), threads + 1).astype(np.int64)
+
+    def part(i):
+        out[cuts[i]:cuts[i + 1]] = np.searchsorted(ascending, values[cuts[i]:cuts[i + 1]], side=side)
+    with ThreadPoolExecutor(threads) as pool:
+        list(pool.map(part, range(threads)))
+    return out
 
 
 def power_law_edges(num_vertex, num_edge, gamma=2.3, seed=1024):
@@ -18,8 +36,8 @@ def power_law_edges(num_vertex, num_edge, gamma=2.3, seed=1024):
     filled = 0
     while filled < num_edge:
         n = num_edge - filled
-        u = np.searchsorted(cdf, rng.random(n), side="right")
-        v = np.searchsorted(cdf, rng.random(n), side="right")
+        u = _search(cdf, rng.random(n), "right")
+        v = _search(cdf, rng.random(n), "right")
         keep = u != v
         m = int(keep.sum())
         out[filled:filled + m, 0] = label[np.minimum(u[keep], num_vertex - 1)]
@@ -44,19 +62,31 @@ def link_prediction_split(edges, portions=(100, 1, 1), seed=1024):
     cum = np.cumsum(portions, dtype=np.float32) / np.sum(portions)
     which = np.searchsorted(cum, rs.rand(len(edges)))
     nodes = np.unique(edges)
-    keys = set((edges[:, 0].astype(np.int64) << 32 | edges[:, 1].astype(np.int64)).tolist())
+    keys = edges[:, 0].astype(np.int64) << 32 | edges[:, 1].astype(np.int64)
+
+    def are_edges(u, v):
+        wanted, place = np.unique(u << 32 | v, return_inverse=True)
+        at = np.minimum(_search(wanted, keys), len(wanted) - 1)
+        found = np.zeros(len(wanted), bool)
+        found[at[wanted[at] == keys]] = True
+        return found[place]
+
     splits = []
     for i in range(1, len(portions)):
         true = edges[which == i]
-        H, T = [], []
-        while len(H) < len(true):
-            u = int(nodes[int(rs.rand() * len(nodes))])
-            v = int(nodes[int(rs.rand() * len(nodes))])
-            if u != v and (u << 32 | v) not in keys and (v << 32 | u) not in keys:
-                H.append(u)
-                T.append(v)
-        splits.append((np.concatenate([true[:, 0], np.asarray(H, edges.dtype)]),
-                       np.concatenate([true[:, 1], np.asarray(T, edges.dtype)]),
+        H, T = np.zeros(0, np.int64), np.zeros(0, np.int64)
+        while len(H) < len(true):  # pairs of draws in their order, many at a time; those behind the last one that is needed go back
+            need = len(true) - len(H)
+            state = rs.get_state()
+            draws = rs.rand(need + need // 50 + 16, 2)
+            u, v = (nodes[(draws[:, side] * len(nodes)).astype(np.int64)].astype(np.int64) for side in (0, 1))
+            good = np.nonzero((u != v) & ~are_edges(u, v) & ~are_edges(v, u))[0][:need]
+            if len(good) == need:
+                rs.set_state(state)
+                rs.rand(good[-1] + 1, 2)
+            H, T = np.concatenate([H, u[good]]), np.concatenate([T, v[good]])
+        splits.append((np.concatenate([true[:, 0], H.astype(edges.dtype)]),
+                       np.concatenate([true[:, 1], T.astype(edges.dtype)]),
                        np.concatenate([np.ones(len(true), np.int64), np.zeros(len(H), np.int64)])))
     return edges[which == 0], splits
 
@@ -105,8 +135,8 @@ def hub_community_edges(num_vertex, num_edge, gamma=2.3, num_community=40, p_in=
     filled = 0
     while filled < num_edge:
         n = num_edge - filled
-        u = np.minimum(np.searchsorted(cdf, rng.random(n), side="right"), num_vertex - 1)
-        v = np.minimum(np.searchsorted(cdf, rng.random(n), side="right"), num_vertex - 1)
+        u = np.minimum(_search(cdf, rng.random(n), "right"), num_vertex - 1)
+        v = np.minimum(_search(cdf, rng.random(n), "right"), num_vertex - 1)
         inside = rng.random(n) < p_in
         r = rng.random(n)
         community = u % K
