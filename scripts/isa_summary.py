@@ -2,8 +2,9 @@
 the instruction mix of the shipped dim-128 training kernel (disassembly of the code object): VGPRs, SGPRs, scratch,
 occupancy, LDS; VALU / VMEM / SALU / DPP counts.
 
-    python scripts/isa_summary.py > profiles/r3/isa_summary.txt
+    python scripts/isa_summary.py > isa_summary.txt
 """
+import glob
 import os
 import re
 import subprocess
@@ -19,12 +20,23 @@ def demangle(names):
     return [o.replace("(anonymous namespace)::", "") for o in out]
 
 
+def sources():
+    """Every file of kernels that the Makefile builds into libgvk.so."""
+    return sorted(os.path.basename(f) for f in glob.glob(os.path.join(CSRC, "*.hip")))
+
+
+def flags():
+    """The Makefile's own flags: what is described is what is built."""
+    with open(os.path.join(CSRC, "Makefile")) as f:
+        line = re.search(r"^FLAGS := (.*)$", f.read(), re.M).group(1)
+    return line.replace("$(ROOT)", ROOT).replace("$(HERE)", CSRC + os.sep).split()
+
+
 def main():
     with tempfile.TemporaryDirectory() as tmp:
-        flags = ["hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-I" + os.path.join(ROOT, "include"), "-I" + CSRC]
         rows = []
-        for source in ("gvk_pairs.hip", "gvk_chains.hip", "gvk_samplers.hip", "gvk_group.hip"):
-            run = subprocess.run(flags + ["-c", os.path.join(CSRC, source), "-o", os.path.join(tmp, source + ".o"),
+        for source in sources():
+            run = subprocess.run(["hipcc"] + flags() + ["-c", os.path.join(CSRC, source), "-o", os.path.join(tmp, source + ".o"),
                                           "-Rpass-analysis=kernel-resource-usage", "--save-temps=obj"], capture_output=True, text=True, cwd=tmp)
             blocks = re.split(r"Function Name: ", run.stderr)[1:]
             for b in blocks:
