@@ -276,7 +276,7 @@ struct table_view {
 // The matrix operand of a tile is 16 rows x 64 bytes; read as that, a load touches 16 cache lines by half and asks the L2 for each
 // twice.  So the two loads of a tile and block take whole lines, eight rows each: lane (r, g) of L0 holds row r % 8, sixteen bytes at
 // 16 g (r < 8) or 64 + 16 g (r >= 8), of L1 the same of row 8 + r % 8; halves of sixteen lanes change places (a DPP move) to make the
-// operands of it.  4096 x 65536 x d512, bf16: 388 -> 338 us together with the order of the workgroups, 1 x 1M x d512: 115 -> 102 us.
+// operands of it.  When it was chosen, 4096 x 65536 x d512, bf16: 388 -> 338 us together with the order of the workgroups, 1 x 1M x d512: 115 -> 102 us.
 //
 // A strip of 256 may end before its last waves begin, and a wave's 64 rows may end inside: both read the table's last row instead, and
 // nothing of what they compute from it is stored.
@@ -366,7 +366,10 @@ __device__ __forceinline__ void change_places(uint4 &l0, uint4 &l1) {
 }
 
 // up to 16 queries: the table is read once and that bounds it.  Each workgroup lays the queries out for itself (no launch
-// before this one) and walks over strips of 64 candidates per wave.
+// before this one) and walks over strips of 64 candidates per wave.  1 x 1M x d128, f32: 22 us (6.0 TB/s), 16 x 1M 31 (6.2).
+// A tile is what its lanes hold, hence 16 queries.  Blocks, against the kernels for many queries with a launch before them: 1 x 10312 x d128
+// 7.1 us against 11.2; d512 8.8 against 11.5, 1 x 100003 13.8 against 15.4, 16 x 100003 16.2 against 16.1, 16 x 1M 122 against 119; with eight
+// blocks (d1024) every workgroup's laying out costs more than the launch: 1 x 100003 26 against 23.5, 16 x 100003 30.5 against 25.
 constexpr int kFewBlocks = 4;  // 512 columns: 16 KB of fragments
 
 template<class Q, class T>
@@ -425,8 +428,8 @@ __global__ void __launch_bounds__(256) few_queries_kernel(const Q *query, int64_
 // memory a read as well: hence the wide stores, and an XCD takes an eighth of the candidates, in order, the parts of a strip one after
 // the other (777 x 99991 f16 on eight outputs in turn: 64 us with 64 candidates of a row at once and strips dealt over the XCDs, 49 with
 // the strips in order, 45 with 256 candidates; 777 x 99968, whose rows begin on lines: 40).
-// 1024 x 1M x d128: f32 817 us, bf16 440; without the table's loads 773 and 395, the stores alone 745 and 380 in any order of them: the write
-// rate of rows (5.5 TB/s) bounds it, and reads between the writes cost more than their bytes.  Waves that stay and walk over
+// 1024 x 1M x d128: f32 816 us, bf16 436; when it was chosen, without the table's loads 773 and 395, the stores alone 745 and 380 in any order of them:
+// the write rate of rows (5.5 TB/s) bounds it, and reads between the writes cost more than their bytes.  Waves that stay and walk over
 // strips with the queries in LDS: 882 and 476.
 // 16 queries x 256 candidates of a workgroup on their way from the waves' registers to memory
 template<class T>
@@ -507,9 +510,9 @@ __global__ void __launch_bounds__(256, ALONE ? 3 : 4) narrow_kernel(const Q *que
 // in LDS, those of the next block and its table rows on their way meanwhile: asked for at the block's start, the scheduler kept from
 // moving them behind the matrix instructions, and first touched when the block is over.  Workgroups stay and take one such square after
 // the other: while the last block of one is multiplied the first of the next is on its way, and the logits are stored behind those loads.
-// 4096 x 65536 x d512 bf16 328 us (838 TFLOP/s; the library's bf16 product of that shape 325), f32 343; a launch per square, with loads
-// where the scheduler put them: 372 and 387.  Of the 328 the 16 squares' four blocks take 200 (d2048: 933 us, 1179 TFLOP/s); the rest is
-// the stores, which a CU's other workgroup overlaps with its own products in part (without stores: 256).
+// 4096 x 65536 x d512 bf16 264 to 282 us from run to run (1040 to 975 TFLOP/s; the library's bf16 product of that shape 307), f32 323; a launch
+// per square, with loads where the scheduler put them: 325 and 367 in the same runs.  d2048: 915 us, 1201 TFLOP/s; a shorter row pays for its
+// stores, which a CU's other workgroup overlaps with its own products in part.
 // Odd numbers of blocks change the buffers' roles from square to square, which takes a build with two squares to a turn.
 template<int TILES>
 constexpr int staying_groups() {  // to a CU: what registers and LDS allow
@@ -724,6 +727,9 @@ int launch_logits(hipStream_t stream, const Q *query, int64_t query_stride, uint
         else                                                                                                                                \
             hipLaunchKernelGGL((logits_kernel<TILES, T, WHOLE, false>), grid, dim3(256), 0, stream, fragments, tiles, num_query, table, logits, logit_stride); \
     }
+    // What is not there is computed all the same, so few tiles take few; what is there is read once for all the tiles of a square.  bf16 logits of 1M
+    // candidates, d256, with two / four / eight tiles to a square: 32 queries 65 / 69 / 77 us, 64 queries 99 / 83 / 87, 128 queries 184 / 129 / 113
+    // (65: 132 / 104 / 89).  A small table is too few squares of eight for the chip: 128 x 10312 x d512 12.4 / 12.7 / 15.1.
     if (!whole) GVK_LOGITS(1, false)
     else if (tiles <= 2) GVK_LOGITS(2, true)
     else if (tiles <= 4) GVK_LOGITS(4, true)

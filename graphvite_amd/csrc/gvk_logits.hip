@@ -34,9 +34,9 @@ __device__ __forceinline__ float reference_of(float largest) { return largest ==
 // k = 64: about 85).  Every lane marks those of its own, a bit each, and puts the chunks they are in into LDS; then they are packed, one
 // addition to the count for a wave.  One slice: they are ranked by counting.  More: they go to a list, and one workgroup per row does the
 // same with the lists.  Rows that defeat the bound (all logits equal, NaN) take the exact way: a bisection of the key, bit by bit.
-// Seven instructions an element, the exponential at a quarter of the rate: 512 x 1M f32 378 us (5.4 TB/s, what reading a row's slices
-// reaches), 1024 x 1M bf16 500 (4.1 TB/s: twice the elements a byte, both count), of those 25 the lists; without collecting at all 350
-// and 400.  Collecting elements one by one as they are met, 450 and 565: four instructions each, and an atomic a round.
+// Seven instructions an element, the exponential at a quarter of the rate: 512 x 1M f32 377 us (5.4 TB/s, what reading a row's slices reaches), 1024 x 1M bf16
+// 395 (5.2 TB/s), of those 21 the lists; calls in a row — one by itself, before the clock is up, takes 470.  When it was chosen, collecting elements one
+// by one as they are met took 450 and 565 against 382 and 490: four instructions each, and an atomic a round.
 constexpr int kTopThreads = 256, kTopWaves = kTopThreads / 64, kMergeThreads = 512, kMergeWaves = kMergeThreads / 64;
 constexpr uint32_t kPacked = 1024;  // keys a workgroup packs
 constexpr uint32_t kKept = 4;       // chunks of a thread kept in LDS; more are read again from memory
@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(kTopThreads) top_kernel(const T *logits, int64
 #pragma unroll
     for (int u = 0; u < U; u++) {
         float x[E];
-        // 16-bit logits are unpacked again, rather than kept unpacked: 78 registers, not 152 (1024 x 1M bf16: 577 us against 631)
+        // 16-bit logits are unpacked again, rather than kept unpacked: 78 registers, not 152 (when it was chosen, 1024 x 1M bf16: 577 us against 631)
         if constexpr (sizeof(T) == 2) asm volatile("" : "+v"(raw[u].x), "+v"(raw[u].y), "+v"(raw[u].z), "+v"(raw[u].w), "+v"(sum));
         else asm volatile("" : "+v"(sum), "+v"(hits[0]), "+v"(hits[kWords - 1]));
         unpack<T>(raw[u], x);
@@ -464,7 +464,7 @@ struct distill_output {
     int64_t grad_stride;
     // workspace of rows longer than a workgroup holds
     float2 *partial;   // [rows][slices]: max and sum
-    float4 *factors;   // [rows]: what the exponent subtracts, w Q / (T S), unused, 1 where there is nothing to learn
+    float4 *factors;   // [rows]: what the exponent subtracts, w Q / (T S), 0 (16 bytes: one load, and what follows stays aligned), 1 where there is nothing to learn
     int32_t *index;    // [rows][k]: candidates with a share of q, each once; -1: none
     float *q;          // [rows][k]: w q / T
 };
@@ -615,8 +615,8 @@ __device__ __forceinline__ void chunk_gradient(const uint4 raw, int place, float
 
 // Rows that fit a workgroup's registers: read once, written once, one launch.  U chunks to a thread.  What bounds many rows is how many of them
 // a CU holds (they wait for their loads and three barriers each): few threads with many chunks, builds near the row's length, the
-// list's entries by their 16-bit place.  4000 x 10312 bf16, a step: 37 us; 1024 threads, 16384 elements and shares of 32 bits: 89.
-// 4000 x 16000 f32 98 (5.2 TB/s) against 134; a few rows are no slower (50 x 10312 f32: 9.5).
+// list's entries by their 16-bit place.  4000 x 10312 bf16, k = 64, a step: 38 us (44 where lists name candidates twice); 1024 threads, 16384 elements and
+// shares of 32 bits, when it was chosen: 89.  4000 x 16000 f32 98 (5.2 TB/s) against 134; a few rows are no slower (50 x 10312 f32: 9.4).
 template<class T, int THREADS, int U, bool GRAD>
 __global__ void __launch_bounds__(THREADS) distill_row_kernel(distill_input in, distill_output out, int64_t first_row) {
     constexpr int E = per_chunk<T>::value, SIZE = THREADS * U * E;
@@ -687,6 +687,8 @@ __global__ void __launch_bounds__(THREADS) distill_row_kernel(distill_input in, 
 
 // Longer rows, in slices: max and sum of every slice; then, a workgroup per row, those joined and the list; then the gradient of every
 // slice, with nothing left to do per row but to find the slice's entries.
+// Slices of 4096 / 8192 / 16384 logits: the loss of 500 x 99991 f16 25.3 / 24.1 / 25.8 us, the step of 512 x 1M bf16 577 / 581 / 562, of 256 x 1M f32
+// 577 / 554 / 561, of 300 x 40000 f32 39.0 / 38.2 / 42.7, of 300 x 20000 bf16 25.6 / 28.0 / 32.2.
 constexpr int kSliceThreads = 256, kSliceElements = 8192;
 
 template<class T>
@@ -836,6 +838,8 @@ int check_temperature(const char *who, float temperature, float *scale) {
 // slices a row of num_col takes wherever in 16 bytes it begins
 int64_t slices_of(int64_t num_col, int64_t slice, int per_chunk) { return (num_col + per_chunk - 1 + slice - 1) / slice; }
 
+// Slices of 8192 / 16384 logits: top 64 of 1024 x 1M bf16 515 / 414 us, of 16 x 1M bf16 40 / 21.7, top 10 of 1000 x 10312 f32 26 / 12.7 (a row is then
+// two slices, two launches); top 100 of 333 x 99991 f32 goes the other way, 37 / 41, and 64 of 1000 x 20000 f32, 35.6 / 40.
 constexpr int64_t kTopSlice = 16384, kTopStep = 4096;
 
 struct top_plan {
@@ -861,6 +865,8 @@ void launch_top(hipStream_t stream, const top_plan &p, const T *logits, int64_t 
                 const top_output &out) {
     constexpr int kChunks = kTopStep / kTopThreads / per_chunk<T>::value;
     const dim3 grid((unsigned)(num_row * p.slices));
+    // One / four maxima to a thread, 333 x 99991 f32: k = 72 39.6 / 40.4 us, 100 41.4 / 42.7, 128 48.6 / 43.8, 200 69.6 / 47.2; 512 x 1M bf16 k = 128
+    // 223 / 228; 333 x 99991 bf16 k = 256 228 / 41 (too many reach the bound then).
 #define GVK_TOP(STEPS)                                                                                                                                              \
     if (k <= 128)                                                                                                                                                  \
         hipLaunchKernelGGL((top_kernel<T, STEPS * kChunks, 1>), grid, dim3(kTopThreads), 0, stream, logits, stride, first_row, (uint32_t)p.slices, num_col, (uint32_t)k, \
@@ -885,7 +891,7 @@ void launch_top(hipStream_t stream, const top_plan &p, const T *logits, int64_t 
     }
 }
 
-constexpr int64_t kRowElements = 16384;  // a row that a workgroup of 1024 threads holds
+constexpr int64_t kRowElements = 16384;  // what the largest build of launch_rows holds: a row of 16381 f32 or 16377 16-bit logits, wherever it begins
 
 int64_t distill_slices(int dtype, int64_t num_col) { return slices_of(num_col, kSliceElements, 16 / (int)size_of(dtype)); }
 

@@ -43,7 +43,7 @@ struct chunked_row {
         return raw;
     }
     // U chunks to a thread, THREADS apart, from chunk0 on: those at chunk1 and behind read as minus infinity.  Only the first and the last can
-    // lie across the row's ends, unless the slice is shorter than that: the others are asked for without a question each (top 64 of
+    // lie across the row's ends, unless the slice is shorter than that: the others are asked for without a question each (when it was chosen, top 64 of
     // 512 x 1M f32: 385 us against 450).
     template<int U, int THREADS>
     __device__ __forceinline__ void load(uint4 (&raw)[U], int64_t chunk0, int64_t chunk1) const {

@@ -1,6 +1,6 @@
 """Thin, typed Python face of the kernel ABI (include/gvk.h) over torch tensors.
 
-torch supplies device memory and streams only; every computation here is a libgvk.so kernel (`scorer.distill` adds two plain torch products).
+torch supplies device memory and streams only; every computation here is a libgvk.so kernel (`scorer.distill` adds three plain torch products).
 A `HipKernels` object is what `solver.GraphSolver` calls; tests for the host logic may inject an object
 (the CPU tests run the engine over tests/hostdev instead: the same entry points served by the CPU oracle).
 """
@@ -142,7 +142,7 @@ class BlockTable(object):
 
     Parameters:
         values (Tensor): uint8 or float8_e4m3fn [rows, >= dim rounded up to 16], a row stride of a multiple of 16 bytes; the
-            columns between dim and that multiple are zero
+            columns between dim and that multiple are zero (whatever they are in a marked block)
         exponents (Tensor): uint8 [rows, (dim + 127) // 128]
         dim (int): columns of a row, 1 to 4096
 

@@ -448,11 +448,12 @@ enum { GVK_F32 = 0, GVK_BF16 = 1, GVK_F16 = 2 };
 
 /* A table of rows in 8 bits:  x[r][c] = value[r][c] * 2^(exponent[r][c / 128] - 127).
  *   values     one e4m3 byte per column (largest magnitude 448, no infinity, 0x7f = NaN); value_stride bytes from row to row, both it and
- *              the pointer multiples of 16; columns dim ... up to a multiple of 16 are part of a row and hold zero
+ *              the pointer multiples of 16; columns dim ... up to a multiple of 16 are part of a row and hold zero (NaN bytes in a marked block)
  *   exponents  one byte per block of 128 columns, [num_row][(dim + 127) / 128]: the least with max |x| <= 448 * 2^(exponent - 127), 127
  *              for a block of zeros, 0 at the least (below 2^-118 or so values round to e4m3's least steps of it);
  *              255 marks a block that held a NaN or an infinity: all of it reads as NaN
- * Values round to nearest, ties to even: off by at most 2^-4 of a value, or 2^-10 * 2^(exponent - 127) for the least ones.
+ * Values round to nearest, ties to even: off by at most 2^-4 of a value, or 2^-10 * 2^(exponent - 127) for the least ones
+ * (above 1.9375 * 2^127 that is 2^128, an infinity as a number of any of the types).
  * num_row up to GVK_MAX_BLOCK_ROWS, dim 1 ... GVK_MAX_BLOCK_DIM, row_stride >= dim elements; rows may have any alignment of their type. */
 int gvk_block_quantize(void *stream, int dtype, const void *rows, int64_t num_row, int dim, int64_t row_stride, uint8_t *values, int64_t value_stride,
                        uint8_t *exponents);
@@ -481,7 +482,7 @@ int gvk_top_logits(void *stream, int dtype, const void *logits, int64_t num_row,
  *     p_j = exp((z_j - m) / temperature) / S                 over all candidates
  *     q_e = exp((t_e - mt) / temperature) / St               mt, St: of the list; with teacher_stats = {mt, log St} of the teacher's whole
  *                                                            row (gvk_top_logits at the same temperature), and Q = sum q_e is below 1
- *     loss[r]    = sum_e q_e (log q_e - log p_{index e})      (unweighted)
+ *     loss[r]    = sum_e q_e (log q_e - log p_{index e})      (unweighted; with Q below 1 the listed part of the divergence, Q log Q at the least)
  *     stats[r]   = {m, log S}                                  what gvk_distill_grad takes
  *     grad[r][j] = weight[r] / temperature * (Q p_j - sum_{e: index e = j} q_e)       weight null: 1
  * `weight` is the derivative by loss[r].  A candidate may be listed more than once: its entries add.  A row without entries, or with every
