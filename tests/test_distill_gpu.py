@@ -64,6 +64,15 @@ def test_a_trained_student_goes_on_from_its_tables(teacher):
     assert len(losses) == 3 and 0 < np.abs(s.vertex_embeddings - before).max() < 1e-2
 
 
+@pytest.mark.parametrize("k", [10, 64])
+def test_a_trained_student_learns_at_the_default_rate(teacher, k):
+    s = student_of(teacher, 64, 3)
+    s.train(model="LINE", num_epoch=200, augmentation_step=2, log_frequency=1 << 30)
+    losses = s.distill(teacher.scorer(), k=k)
+    print("losses", losses)
+    assert np.isfinite(losses).all() and losses[-1] < losses[0]
+
+
 def test_the_same_seed_the_same_student(teacher):
     scorer = teacher.scorer()
     a, b = student_of(teacher), student_of(teacher)
